@@ -236,6 +236,93 @@ WKV6_API int wkv6_softmax_xent_bf16(int64_t rows, int32_t V, void *logits_inout,
 WKV6_API int wkv6_scale_bf16(int64_t n, void *g, const float *scale, void *stream);
 
 /*
+ * Log-probabilities of given tokens, and the losses on them that a model is trained with after pre-training.  No counterpart in the
+ * reference (its trainer files are empty).  S sequences of T tokens: token (s, t) has its V logits at
+ * logits + s * seq_stride + t * row_stride (elements; 0 selects the dense value), the rest is dense [S, T].
+ *   lp = z_a / temperature - log sum_j exp(z_j / temperature), fp32 arithmetic
+ * A token whose mask is 0 or whose target lies outside [0, V) does not count: its logits are not read, its log-probability is 0, and
+ * its gradient is zeros.  Gradients are dense [S, T, V] of `dtype` and must not overlap the logits.
+ */
+typedef struct {
+    int32_t S, T, V;
+    int32_t dtype;                       /* logits and their gradient: WKV6_BF16, WKV6_F16, WKV6_F32; aligned to one element */
+    float temperature;                   /* > 0 */
+    int64_t seq_stride, row_stride;
+    const void *logits;
+    const int64_t *targets;
+    const uint8_t *mask;                 /* one byte per token, or NULL: all count */
+} wkv6_token_logits;
+
+/* log_probs [S, T] fp32.  stat (optional, fp32 [S, T, 2], 8-byte aligned) is what the backward needs of a row. */
+WKV6_API int wkv6_token_log_probs(const wkv6_token_logits *p, float *log_probs, float *stat, void *stream);
+/* g = coefficient * (*factor) * d lp / d logits, one coefficient per token ([S, T]) or per sequence ([S], per_sequence != 0); factor
+ * (one fp32 value on the device) may be NULL.  unless_one: nothing is done where *factor is 1. */
+WKV6_API int wkv6_token_log_probs_backward(const wkv6_token_logits *p, const float *stat, const float *coefficient, int32_t per_sequence,
+                                           const float *factor, int32_t unless_one, void *g, void *stream);
+
+/* Clipped policy loss:  ratio = exp(lp - old),  d = ref - lp,
+ *   loss = scale * sum of w * ( -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1) )
+ * over the tokens that count, w = 1 / their number (WKV6_MEAN), 1 / (S * their number in the sequence) (WKV6_SEQUENCE_MEAN) or 1
+ * (WKV6_SUM).  Without such a token the loss is 0.
+ *   g (optional) receives the gradient of the logits in the same pass; stat (optional) and coefficient [S, T] (= d loss / d lp) are what
+ *   wkv6_token_log_probs_backward needs to form it again, times a factor.
+ * workspace: wkv6_policy_loss_workspace_bytes(S, T, reduction) bytes.  Sums run in a fixed order. */
+enum { WKV6_MEAN = 0, WKV6_SEQUENCE_MEAN = 1, WKV6_SUM = 2 };
+typedef struct {
+    const float *advantages, *old_log_probs;   /* [S, T] */
+    const float *ref_log_probs;                /* [S, T]; may be NULL when kl_coef is 0 */
+    double clip_low, clip_high, kl_coef, scale;
+    int32_t reduction;
+} wkv6_policy;
+WKV6_API size_t wkv6_policy_loss_workspace_bytes(int32_t S, int32_t T, int32_t reduction);
+WKV6_API int wkv6_policy_loss(const wkv6_token_logits *p, const wkv6_policy *c, float *loss, float *log_probs, float *stat,
+                              float *coefficient, void *g, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Loss of paired log ratios behind wkv6_token_log_probs: sequence i is preferred to sequence i + S / 2,
+ *   L_s = sum (average: mean) of lp over the sequence,   D = beta ((L_i - ref_i) - (L_j - ref_j)) - margin,
+ *   loss = scale * mean over the pairs of  -(1 - label_smoothing) log sigmoid(D) - label_smoothing log sigmoid(-D)
+ * sequence_log_probs [S] = L; coefficient [S] = d loss / d lp of the sequence's tokens (for wkv6_token_log_probs_backward,
+ * per_sequence = 1).  p's logits are not read.  workspace: wkv6_preference_loss_workspace_bytes(S) bytes, 8-byte aligned. */
+typedef struct {
+    const float *ref_log_probs;                /* [S] or NULL (zeros) */
+    double beta, label_smoothing, margin, scale;
+    int32_t average;
+} wkv6_preference;
+WKV6_API size_t wkv6_preference_loss_workspace_bytes(int32_t S);
+WKV6_API int wkv6_preference_loss(const wkv6_token_logits *p, const float *log_probs, const wkv6_preference *c, float *loss,
+                                  float *sequence_log_probs, float *coefficient, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * AdamW over many tensors at once, in place.  For every value, in fp32 (g' = g * (*grad_scale)):
+ *   m <- beta1 m + (1 - beta1) g',   v <- beta2 v + (1 - beta2) g'^2
+ *   p <- p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * state_bits 32: m and v are fp32.  8: blocks of 256 values, counted from the tensor's first, share a scale (one fp32 value per block):
+ * m = code * m_scale and sqrt(v) = code * v_scale with e4m3 codes, the scale 1/448 of the block's largest value; m is rounded to
+ * nearest, sqrt(v) up or down with the probabilities that keep its mean (an optimizer step changes it by less than half an e4m3
+ * step).  stochastic: bf16 parameters are rounded the same way, from 16 random bits each; otherwise to nearest.  The random bits are
+ * a function of seed, t, the tensor's `index` and the value's place in it.
+ * A gradient that is infinite or NaN makes its value NaN (8 bits: its block's moments too).
+ * t is `step`, or *step_device where that is not NULL; lr is `lr`, or *lr_device.  Tensors must not overlap; n == 0 is allowed.
+ * No counterpart in the reference (its trainer files are empty).
+ */
+typedef struct {
+    void *p;                             /* BF16 or F32 (the call's dtype), as g */
+    const void *g;
+    void *m, *v;
+    float *m_scale, *v_scale;            /* 8 bits: [(n + 255) / 256] */
+    int64_t n;
+    int64_t index;                       /* in [0, 2^31) */
+} wkv6_adamw_tensor;
+typedef struct {
+    int32_t dtype, state_bits, stochastic;
+    int64_t step, seed;
+    double lr, beta1, beta2, eps, weight_decay;
+    const int64_t *step_device;
+    const float *lr_device, *grad_scale; /* one value each, or NULL */
+} wkv6_adamw;
+WKV6_API int wkv6_adamw_step(const wkv6_adamw *c, int64_t count, const wkv6_adamw_tensor *tensors, void *stream);
+
+/*
  * Sequence splitting along T (no counterpart in the reference, whose kernels cap T at a compile-time constant and
  * never split a sequence; sequences of 131072 tokens need it).  A sequence cut into G segments is
  * handled as a batch of B*G shorter sequences (a dense [B, G*Tseg, C] tensor is a [B*G, Tseg, C] tensor) whose

@@ -27,6 +27,8 @@ SYMBOLS = (
     "wkv6_groupnorm_silu_gate_forward", "wkv6_groupnorm_silu_gate_backward",
     "wkv6_shift_mix_forward", "wkv6_shift_mix_backward", "wkv6_shift_mix_workspace_bytes", "wkv6_shift_mix_pair_forward", "wkv6_shift_mix_pair_backward",
     "wkv6_lora_mix_forward", "wkv6_lora_mix_backward",
+    "wkv6_token_log_probs", "wkv6_token_log_probs_backward", "wkv6_policy_loss", "wkv6_policy_loss_workspace_bytes",
+    "wkv6_preference_loss", "wkv6_preference_loss_workspace_bytes", "wkv6_adamw_step",
     "wkv6_layer_norm_forward", "wkv6_layer_norm_backward", "wkv6_layer_norm_workspace_bytes", "wkv6_copy_2d_async",
     "wkv6_relu_sq_forward", "wkv6_relu_sq_backward", "wkv6_sigmoid_mul_forward", "wkv6_sigmoid_mul_backward",
     "wkv6_xla_forward", "wkv6_xla_backward", "wkv6_xla_forward_with_state", "wkv6_xla_forward_ckpt", "wkv6_xla_backward_ws",
@@ -41,6 +43,39 @@ class Problem(ctypes.Structure):
         ("gu_dtype", ctypes.c_int32), ("s_dtype", ctypes.c_int32), ("variant", ctypes.c_int32),
         ("row_stride", ctypes.c_int64), ("batch_stride", ctypes.c_int64),
     ]
+
+
+class TokenLogits(ctypes.Structure):
+    _fields_ = [
+        ("S", ctypes.c_int32), ("T", ctypes.c_int32), ("V", ctypes.c_int32), ("dtype", ctypes.c_int32), ("temperature", ctypes.c_float),
+        ("seq_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+        ("logits", ctypes.c_void_p), ("targets", ctypes.c_void_p), ("mask", ctypes.c_void_p),
+    ]
+
+
+class Policy(ctypes.Structure):
+    _fields_ = [
+        ("advantages", ctypes.c_void_p), ("old_log_probs", ctypes.c_void_p), ("ref_log_probs", ctypes.c_void_p),
+        ("clip_low", ctypes.c_double), ("clip_high", ctypes.c_double), ("kl_coef", ctypes.c_double), ("scale", ctypes.c_double),
+        ("reduction", ctypes.c_int32),
+    ]
+
+
+class Preference(ctypes.Structure):
+    _fields_ = [
+        ("ref_log_probs", ctypes.c_void_p), ("beta", ctypes.c_double), ("label_smoothing", ctypes.c_double),
+        ("margin", ctypes.c_double), ("scale", ctypes.c_double), ("average", ctypes.c_int32),
+    ]
+
+
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("p", "g", "m", "v", "m_scale", "v_scale")] + [("n", ctypes.c_int64), ("index", ctypes.c_int64)]
+
+
+class AdamWConfig(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_int32) for n in ("dtype", "state_bits", "stochastic")] + [("step", ctypes.c_int64), ("seed", ctypes.c_int64)]
+                + [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+                + [(n, ctypes.c_void_p) for n in ("step_device", "lr_device", "grad_scale")])
 
 
 class WKV6Error(RuntimeError):
@@ -142,6 +177,21 @@ def _load():
     lib.wkv6_layer_norm_workspace_bytes.argtypes = [i64, i32]
     lib.wkv6_layer_norm_backward.restype = ctypes.c_int
     lib.wkv6_layer_norm_backward.argtypes = [i64, i32] + [vp] * 9 + [sz, vp]
+    rows = ctypes.POINTER(TokenLogits)
+    lib.wkv6_token_log_probs.restype = ctypes.c_int
+    lib.wkv6_token_log_probs.argtypes = [rows, vp, vp, vp]
+    lib.wkv6_token_log_probs_backward.restype = ctypes.c_int
+    lib.wkv6_token_log_probs_backward.argtypes = [rows, vp, vp, i32, vp, i32, vp, vp]
+    lib.wkv6_policy_loss_workspace_bytes.restype = sz
+    lib.wkv6_policy_loss_workspace_bytes.argtypes = [i32] * 3
+    lib.wkv6_policy_loss.restype = ctypes.c_int
+    lib.wkv6_policy_loss.argtypes = [rows, ctypes.POINTER(Policy)] + [vp] * 6 + [sz, vp]
+    lib.wkv6_preference_loss_workspace_bytes.restype = sz
+    lib.wkv6_preference_loss_workspace_bytes.argtypes = [i32]
+    lib.wkv6_preference_loss.restype = ctypes.c_int
+    lib.wkv6_preference_loss.argtypes = [rows, vp, ctypes.POINTER(Preference)] + [vp] * 4 + [sz, vp]
+    lib.wkv6_adamw_step.restype = ctypes.c_int
+    lib.wkv6_adamw_step.argtypes = [ctypes.POINTER(AdamWConfig), i64, ctypes.POINTER(AdamWTensor), vp]
     vpp = ctypes.POINTER(vp)
     lib.wkv6_lora_mix_forward.restype = ctypes.c_int
     lib.wkv6_lora_mix_forward.argtypes = [i32] * 3 + [vp] * 4 + [vpp, vp]

@@ -1,0 +1,217 @@
+"""AdamW for the training step: one launch per parameter type updates all tensors of a model (C ABI ``wkv6_adamw_step``).
+
+``AdamW`` is a ``torch.optim.Optimizer``; ``adamw_step`` is the update behind it, on lists of tensors.  What they add to the
+framework's optimizer: moments in fp32 whatever the parameters' type (a bf16 moment cannot follow beta2 = 0.999: a step changes it by
+less than half its last bit), moments in 8 bits (2.03 bytes per value instead of 8), and stochastic rounding of bf16 parameters, which
+keeps the updates that are smaller than half a parameter's last bit on average, without an fp32 copy of the parameters.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from ._lib import AdamWConfig, AdamWTensor, check, lib
+from .ops import _DT, _check_cuda, _ptr, _stream
+
+BLOCK = 256      # values that share a scale where states have 8 bits
+
+
+def _overlap(ts):
+    """Whether two of the tensors share memory."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in ts if t.numel())
+    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+
+
+def _check_lists(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales):
+    if (m_scales is None) != (v_scales is None):
+        raise ValueError("states in 8 bits need the scales of both moments")
+    lists = [l for l in (params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales) if l is not None]
+    if any(len(l) != len(params) for l in lists):
+        raise ValueError("all lists must have one tensor per parameter")
+    if not params:
+        return
+    state = torch.float32 if m_scales is None else torch.float8_e4m3fn
+    dev = params[0].device
+    for l in lists:
+        _check_cuda(*l)
+    for i, p in enumerate(params):
+        if p.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"parameter {i} must be bf16 or fp32, not {p.dtype}")
+        if grads[i].dtype != p.dtype:
+            raise TypeError(f"gradient {i} must be {p.dtype} as its parameter, not {grads[i].dtype}")
+        for t in (exp_avgs[i], exp_avg_sqs[i]):
+            if t.dtype != state:
+                raise TypeError(f"the moments of parameter {i} must be {state}, not {t.dtype}")
+        for t in (grads[i], exp_avgs[i], exp_avg_sqs[i]):
+            if t.numel() != p.numel():
+                raise ValueError(f"parameter {i} has {p.numel()} values, its gradient or a moment {t.numel()}")
+        if m_scales is not None:
+            for t in (m_scales[i], v_scales[i]):
+                if t.dtype != torch.float32 or t.numel() != -(-p.numel() // BLOCK):
+                    raise ValueError(f"the scales of parameter {i} must be fp32, one per {BLOCK} values")
+        for l in lists:
+            if l[i].device != dev:
+                raise ValueError("all tensors must be on one device")
+            if l[i].layout != torch.strided or not l[i].is_contiguous():
+                raise ValueError(f"tensor {i} of a list is not contiguous")
+    if _overlap([t for l in lists if l is not grads for t in l]):
+        raise ValueError("parameters, moments and scales must not share memory")
+
+
+def _device_value(t, dtype, name, dev):
+    if t.dtype != dtype or t.numel() != 1 or t.device != dev:
+        raise ValueError(f"{name} must be one {dtype} value on the parameters' device")
+    return t.data_ptr()
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp_avg_sq_scales=None, step, lr=1e-3,
+               betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, seed: int = 0, stochastic_rounding: bool = True,
+               grad_scale: torch.Tensor | None = None, first_index: int = 0) -> None:
+    """One AdamW step over lists of tensors, in place: m <- beta1 m + (1 - beta1) g, v <- beta2 v + (1 - beta2) g^2,
+    p <- p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps), all in fp32.
+
+    ``params``: bf16 or fp32, contiguous, both types in one list if need be; ``grads`` of their types.
+    ``exp_avgs``, ``exp_avg_sqs``: fp32; or, with ``exp_avg_scales`` and ``exp_avg_sq_scales`` (fp32, one per 256 values counted from the
+    tensor's first), float8_e4m3fn codes: m = code * scale, sqrt(v) = code * scale.  New states are zeros in either form.
+    ``step``: t of this step, counted from 1; an int, or one int64 value on the device (a captured step reads it at every replay, an
+    int would stay what it was).  ``lr``: a float, or one fp32 value on the device.
+    ``grad_scale``: one fp32 value on the device that multiplies the gradients (clipping, loss scaling).
+    ``stochastic_rounding``: bf16 parameters are rounded up or down with the probabilities that keep their mean, else to nearest.  The
+    random bits (also of 8-bit states) follow from ``seed``, the step, and the tensor's and the value's positions: the tensor's is
+    its place in the list plus ``first_index``."""
+    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    m_scales = None if exp_avg_scales is None else list(exp_avg_scales)
+    v_scales = None if exp_avg_sq_scales is None else list(exp_avg_sq_scales)
+    _check_lists(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales)
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+        raise ValueError("betas must lie in [0, 1)")
+    if not (math.isfinite(eps) and eps >= 0.0 and math.isfinite(weight_decay)):
+        raise ValueError("eps must not be negative, eps and weight_decay must be finite")
+    if not params:
+        return
+    dev = params[0].device
+    c = AdamWConfig()
+    c.state_bits, c.stochastic, c.seed = 32 if m_scales is None else 8, bool(stochastic_rounding), seed
+    c.beta1, c.beta2, c.eps, c.weight_decay = *betas, eps, weight_decay
+    if isinstance(step, torch.Tensor):
+        c.step_device = _device_value(step, torch.int64, "step", dev)
+    else:
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("a captured step needs its number on the device: an int would be the same at every replay")
+        if step < 1:
+            raise ValueError("steps are counted from 1")
+        c.step = step
+    if isinstance(lr, torch.Tensor):
+        c.lr_device = _device_value(lr, torch.float32, "lr", dev)
+    else:
+        if not math.isfinite(lr):
+            raise ValueError("lr must be finite")
+        c.lr = lr
+    if grad_scale is not None:
+        c.grad_scale = _device_value(grad_scale, torch.float32, "grad_scale", dev)
+    none = [None] * len(params)
+    with torch.cuda.device(dev), torch.no_grad():
+        for dtype in (torch.bfloat16, torch.float32):
+            which = [i for i, p in enumerate(params) if p.dtype == dtype]
+            if not which:
+                continue
+            table = (AdamWTensor * len(which))()
+            for e, i in zip(table, which):
+                e.p, e.g, e.m, e.v = params[i].data_ptr(), grads[i].data_ptr(), exp_avgs[i].data_ptr(), exp_avg_sqs[i].data_ptr()
+                if m_scales is not None:
+                    e.m_scale, e.v_scale = m_scales[i].data_ptr(), v_scales[i].data_ptr()
+                e.n, e.index = params[i].numel(), first_index + i
+            c.dtype = _DT[dtype]
+            check(lib.wkv6_adamw_step(c, len(which), table, _stream(dev)))
+    for l in (params, exp_avgs, exp_avg_sqs, m_scales or (), v_scales or ()):
+        for t in l:
+            torch.autograd.graph.increment_version(t)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over bf16 and fp32 parameters on CUDA devices, each group's in one launch per type (see ``adamw_step``).
+
+    ``state_bits``: 32 (fp32 moments) or 8 (e4m3 codes and a scale per 256 values).  ``stochastic_rounding``, ``seed``: how bf16
+    parameters are rounded.  ``lr`` may be a tensor (one fp32 value on the parameters' device).
+    ``grad_scale``: an attribute, None or one fp32 value on the device that multiplies the gradients of the next steps.
+    ``capturable``: the step number is kept on the device (one per group), so that ``step`` can be captured into a CUDA graph; every
+    parameter that gets gradients must then get them from its group's first step on.  A float ``lr`` stays in a captured step as it was.
+    ``state_dict`` holds the moments in their own types; ``load_state_dict`` keeps them (parameters do not lend them theirs)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32,
+                 stochastic_rounding: bool = True, seed: int = 0, capturable: bool = False):
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        if not isinstance(lr, torch.Tensor) and not (math.isfinite(lr) and lr >= 0.0):
+            raise ValueError("lr must be finite and not negative")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError("betas must lie in [0, 1)")
+        if not (math.isfinite(eps) and eps >= 0.0 and math.isfinite(weight_decay) and weight_decay >= 0.0):
+            raise ValueError("eps and weight_decay must be finite and not negative")
+        self.grad_scale = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      stochastic_rounding=stochastic_rounding, seed=seed, capturable=capturable, step=None))
+
+    def _state_of(self, p, group):
+        s = self.state[p]
+        if not s:
+            if group["capturable"] and group["step"] is not None:
+                raise RuntimeError("a capturable group's parameters must have gradients from its first step on")
+            if group["state_bits"] == 32:
+                s["exp_avg"], s["exp_avg_sq"] = (torch.zeros(p.shape, dtype=torch.float32, device=p.device) for _ in range(2))
+            else:
+                for key in ("exp_avg", "exp_avg_sq"):
+                    s[key] = torch.zeros(p.shape, dtype=torch.float8_e4m3fn, device=p.device)
+                    s[key + "_scale"] = torch.zeros(-(-p.numel() // BLOCK), dtype=torch.float32, device=p.device)
+            s["step"] = 0
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        first = 0
+        for group in self.param_groups:
+            # parameters of one launch: on one device, and at one step (a parameter that had no gradient before is behind)
+            batches = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW does not take sparse gradients")
+                s = self._state_of(p, group)
+                batches.setdefault((p.device, s["step"]), []).append((p, s))
+            for (device, at), batch in batches.items():
+                if group["capturable"]:
+                    if group["step"] is None:
+                        group["step"] = torch.zeros((), dtype=torch.int64, device=device)
+                    elif group["step"].device != device:
+                        raise RuntimeError("a capturable group's parameters must be on one device")
+                    group["step"].add_(1)
+                ps, ss = [p for p, _ in batch], [s for _, s in batch]
+                scales = ([s[k + "_scale"] for s in ss] for k in ("exp_avg", "exp_avg_sq")) if group["state_bits"] == 8 else (None, None)
+                m_scales, v_scales = scales
+                adamw_step(ps, [p.grad.contiguous() for p in ps], [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss],
+                           exp_avg_scales=m_scales, exp_avg_sq_scales=v_scales,
+                           step=group["step"] if group["capturable"] else at + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                           weight_decay=group["weight_decay"], seed=group["seed"], stochastic_rounding=group["stochastic_rounding"],
+                           grad_scale=self.grad_scale, first_index=first)
+                if not group["capturable"]:
+                    for s in ss:
+                        s["step"] = at + 1
+                first += len(ps)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        own = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, own):
+            for key, x in state_dict["state"].get(i, {}).items():
+                self.state[p][key] = x.detach().to(p.device, copy=True) if isinstance(x, torch.Tensor) else x
+        for group in self.param_groups:
+            if isinstance(group["step"], torch.Tensor) and group["params"]:
+                group["step"] = group["step"].to(group["params"][0].device, copy=True)
