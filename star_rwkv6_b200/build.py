@@ -1,5 +1,5 @@
 """Build the CUDA library in-tree: star_rwkv6_b200/libwkv6_b200.so (sm_100a only), and the native call path of the torch
-operator: star_rwkv6_b200/_native.so (csrc/wkv6_torch.cpp, host code against the installed torch).
+operator and of the losses and the optimizer step: star_rwkv6_b200/_native.so (csrc/wkv6_torch*.cpp, host code against the installed torch).
 
 ``python star_rwkv6_b200/build.py`` (run as a script, so that it works before the library exists) compiles every ``.cu`` under ``csrc/`` with nvcc and links
 one shared object that exports the C ABI declared in ``include/wkv6_b200.h``.  nvcc
@@ -52,7 +52,7 @@ def native_command():
     inc = [os.path.join(torch_dir, "include"), os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
            os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"] + ["-I" + d for d in inc]
-            + [os.path.join(CSRC, "wkv6_torch.cpp"), "-o", NATIVE, "-L" + os.path.join(torch_dir, "lib")]
+            + [os.path.join(CSRC, f) for f in ("wkv6_torch.cpp", "wkv6_torch_training.cpp")] + ["-o", NATIVE, "-L" + os.path.join(torch_dir, "lib")]
             + ["-l" + n for n in ("torch_python", "torch", "torch_cpu", "torch_cuda", "c10", "c10_cuda", "dl")])
 
 

@@ -6,28 +6,11 @@
 // Python autograd node with zero-filled gradients for the checkpoint buffer) took 27 us and 300 us.  Every function
 // here returns None when the call is not the plain one it handles - other tensor types, a tracing or dispatch mode,
 // layouts or arguments that need a conversion or an error message - and the Python path then runs instead.
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/grad_mode.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-#include <torch/csrc/Exceptions.h>
-#include <ATen/ATen.h>
-#include <ATen/core/dispatch/Dispatcher.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <dlfcn.h>
-
-#include "../../include/wkv6_b200.h"
+#include "wkv6_torch.h"
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
+using namespace wkv6_native;
 
 // The library is the one the Python side loaded (WKV6_B200_LIB may select another build of it).
 struct Api {
@@ -47,33 +30,8 @@ struct Api {
     bool bound = false;
 } api;
 
-int dtype_code(at::ScalarType t) {
-    switch (t) {
-        case at::kBFloat16: return WKV6_BF16;
-        case at::kHalf: return WKV6_F16;
-        case at::kFloat: return WKV6_F32;
-        default: return -1;
-    }
-}
-
 // fp16 inputs give fp32 outputs and gradients, as in the reference operator
 at::ScalarType result_type(at::ScalarType x) { return x == at::kHalf ? at::kFloat : x; }
-
-bool plain_mode() {
-    return api.bound && !c10::impl::TorchDispatchModeTLS::any_modes_set() && !at::impl::torch_function_mode_enabled() &&
-           !torch::jit::tracer::isTracing();
-}
-
-// A strided CUDA tensor that is what its memory holds: not wrapped by a transform, no lazy negation.
-bool plain_storage(const Tensor &t) {
-    constexpr c10::DispatchKeySet odd({c10::DispatchKey::Python, c10::DispatchKey::Batched, c10::DispatchKey::FuncTorchBatched,
-                                       c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize,
-                                       c10::DispatchKey::Conjugate, c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor});
-    return t.defined() && t.is_cuda() && t.layout() == at::kStrided && t.has_storage() && (t.key_set() & odd).empty();
-}
-
-// ... and of the exact class Tensor (or Parameter).
-bool plain_tensor(PyObject *o) { return THPVariable_CheckExact(o) && plain_storage(THPVariable_Unpack(o)); }
 
 struct Call {
     wkv6_problem p{};
@@ -124,10 +82,6 @@ Tensor like(const Tensor &r, at::ScalarType t, bool dense) {   // one stride set
     return dense ? at::detail::empty_cuda(r.sizes(), t, r.device(), std::nullopt)
                  : at::detail::empty_strided_cuda(r.sizes(), r.strides(), t, r.device());
 }
-
-Tensor bytes(size_t n, const Tensor &r) { return at::detail::empty_cuda({(int64_t)n}, at::kByte, r.device(), std::nullopt); }
-
-void *stream_of(const Tensor &r) { return c10::cuda::getCurrentCUDAStream(r.device().index()).stream(); }
 
 // The forward without a checkpoint, split where the library says so; `states` receives the segments' entering states.
 int run_forward(const Call &c, const Tensor &r, const Tensor &k, const Tensor &v, const Tensor &w, const Tensor &u, Tensor &y,
@@ -239,14 +193,12 @@ struct WKV6Function : public torch::autograd::Function<WKV6Function> {
     }
 };
 
-PyObject *none() { Py_RETURN_NONE; }
-
 #define ARG(i) THPVariable_Unpack(args[i])
 
 // wkv6(r, k, v, w, u, head_size, variant, cut = True) -> y or None
 PyObject *py_wkv6(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if ((n != 7 && n != 8) || !plain_mode()) return none();
+    if ((n != 7 && n != 8) || !api.bound || !plain_mode()) return none();
     for (int i = 0; i < 5; ++i)
         if (!plain_tensor(args[i])) return none();
     const int64_t N = PyLong_AsLongLong(args[5]), variant = PyLong_AsLongLong(args[6]);
@@ -277,7 +229,7 @@ PyObject *py_wkv6(PyObject *, PyObject *const *args, Py_ssize_t n) {
 // with_state(r, k, v, w, u, init_state or None, head_size, variant, cut = True) -> (y, state) or None
 PyObject *py_with_state(PyObject *, PyObject *const *args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if ((n != 8 && n != 9) || !plain_mode()) return none();
+    if ((n != 8 && n != 9) || !api.bound || !plain_mode()) return none();
     for (int i = 0; i < 5; ++i)
         if (!plain_tensor(args[i])) return none();
     const int64_t N = PyLong_AsLongLong(args[6]), variant = PyLong_AsLongLong(args[7]);
@@ -337,14 +289,15 @@ PyObject *py_bind(PyObject *, PyObject *arg) {
     SYM(split_segments) SYM(split_state_bytes) SYM(split_workspace_bytes) SYM(forward_split) SYM(backward_split)
     SYM(resolve_variant) SYM(last_error)
 #undef SYM
+    if (const char *missing = bind_training(h)) return PyErr_Format(PyExc_ImportError, "%s lacks %s", path, missing);
     api.bound = true;
     Py_RETURN_NONE;
 }
 
+#define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     {"bind", py_bind, METH_O, nullptr},
-    {"wkv6", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_wkv6)), METH_FASTCALL, nullptr},
-    {"with_state", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_with_state)), METH_FASTCALL, nullptr},
+    METHOD(wkv6), METHOD(with_state), METHOD(token_log_probs), METHOD(policy_loss), METHOD(preference_loss), METHOD(adamw_step),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -22,7 +22,7 @@ import math
 import torch
 
 from ._lib import Policy, Preference, TokenLogits, check, lib
-from .ops import _DT, _check_cuda, _ptr, _stream
+from .ops import _DT, _check_cuda, _native, _ptr, _stream
 
 
 class _LMLoss(torch.autograd.Function):
@@ -163,6 +163,9 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, mask: torch.Ten
                     temperature: float = 1.0) -> torch.Tensor:
     """log softmax(logits / temperature) at the given tokens: fp32 of the shape of ``targets`` (int64), for logits [*targets.shape, V].
     ``mask``: bool of the same shape, True where a token counts.  Differentiable with respect to the logits."""
+    lp = _native.token_log_probs(logits, targets, mask, temperature)
+    if lp is not None:
+        return lp
     _check_targets(logits, targets, mask, temperature)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _TokenLogProbs.apply(logits, targets, mask, temperature)
@@ -229,7 +232,6 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
     ``scale`` multiplies the loss and its gradient.  The logit gradient is computed along with the loss, in one pass, for a loss that
     is the end of the graph: a factor applied to the loss afterwards costs a second pass, one given here does not.
     ``log_probs`` carries no gradient."""
-    _check_targets(logits, targets, mask, temperature)
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {', '.join(_REDUCTIONS)}, not {reduction!r}")
     if not (0.0 <= clip_low <= 1.0 and clip_high >= 0.0):
@@ -238,6 +240,11 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
         raise ValueError("kl_coef must be finite and not negative, scale finite")
     if kl_coef > 0.0 and ref_log_probs is None:
         raise ValueError("a KL term needs ref_log_probs")
+    out = _native.policy_loss(logits, targets, mask, advantages, old_log_probs, ref_log_probs, temperature, clip_low, clip_high, kl_coef,
+                              scale, _REDUCTIONS[reduction])
+    if out is not None:
+        return out
+    _check_targets(logits, targets, mask, temperature)
     consts = (_per_token(advantages, "advantages", targets), _per_token(old_log_probs, "old_log_probs", targets),
               _per_token(ref_log_probs, "ref_log_probs", targets) if ref_log_probs is not None else None)
     args = (logits, targets, mask, temperature, consts, (clip_low, clip_high, kl_coef, scale), _REDUCTIONS[reduction])
@@ -292,13 +299,16 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_log_probs: 
     ``-(1 - label_smoothing) * log sigmoid(D) - label_smoothing * log sigmoid(-D)``, times ``scale``.
     A sequence without a token that counts has L = 0; without a pair the loss is 0.
     ``sequence_log_probs`` [2P] carries no gradient (rewards: beta * (L - R))."""
-    _check_targets(logits, targets, mask, 1.0)
     if targets.dim() != 2 or targets.shape[0] % 2:
         raise ValueError(f"targets must be [2P, T], the preferred sequences first, not {tuple(targets.shape)}")
     if not (math.isfinite(beta) and beta > 0.0 and math.isfinite(margin) and math.isfinite(scale)):
         raise ValueError("beta must be positive and finite, margin and scale finite")
     if not 0.0 <= label_smoothing < 1.0:
         raise ValueError("label_smoothing must lie in [0, 1)")
+    out = _native.preference_loss(logits, targets, mask, ref_log_probs, beta, label_smoothing, margin, scale, bool(average))
+    if out is not None:
+        return out
+    _check_targets(logits, targets, mask, 1.0)
     ref = None if ref_log_probs is None else _per_token(ref_log_probs, "ref_log_probs", targets[:, 0] if targets.shape[1] else targets.sum(1))
     args = (logits, targets, mask, ref, (beta, label_smoothing, margin, scale), bool(average))
     if torch.is_grad_enabled() and logits.requires_grad:

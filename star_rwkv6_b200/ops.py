@@ -30,7 +30,7 @@ except ImportError as e:
 
     class _native:
         """Leaves every call to the Python path, as the module does with calls that it does not handle."""
-        wkv6 = with_state = staticmethod(lambda *args: None)
+        wkv6 = with_state = token_log_probs = policy_loss = preference_loss = adamw_step = staticmethod(lambda *args: None)
 
 _DT = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
 

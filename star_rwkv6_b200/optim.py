@@ -12,7 +12,7 @@ import math
 import torch
 
 from ._lib import AdamWConfig, AdamWTensor, check, lib
-from .ops import _DT, _check_cuda, _ptr, _stream
+from .ops import _DT, _check_cuda, _native, _ptr, _stream
 
 BLOCK = 256      # values that share a scale where states have 8 bits
 
@@ -83,6 +83,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp
     params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
     m_scales = None if exp_avg_scales is None else list(exp_avg_scales)
     v_scales = None if exp_avg_sq_scales is None else list(exp_avg_sq_scales)
+    if _native.adamw_step(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales, step, lr, betas[0], betas[1], eps, weight_decay, seed,
+                          bool(stochastic_rounding), grad_scale, first_index):
+        return
     _check_lists(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales)
     if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
         raise ValueError("betas must lie in [0, 1)")
@@ -126,7 +129,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp
             check(lib.wkv6_adamw_step(c, len(which), table, _stream(dev)))
     for l in (params, exp_avgs, exp_avg_sqs, m_scales or (), v_scales or ()):
         for t in l:
-            torch.autograd.graph.increment_version(t)
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)
 
 
 class AdamW(torch.optim.Optimizer):
