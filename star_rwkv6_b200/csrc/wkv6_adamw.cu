@@ -1,12 +1,12 @@
 // AdamW over many tensors at once (include/wkv6_b200.h gives the formulas), states in fp32 or in blocks of 256 e4m3 codes with a scale.
 //
 // Bound by HBM: a bf16 value with fp32 states moves 22 bytes, with 8-bit states 10.06, for about twenty operations.  The tensors of a
-// model differ in size by four orders of magnitude, so they are cut into chunks of 4096 values and the blocks of one launch walk all
+// model differ in size by four orders of magnitude, so they are cut into chunks of 2048 values and the blocks of one launch walk all
 // chunks; a chunk's tensor is found by bisection in a table that travels in the launch's arguments (no copy to the device, nothing to
 // keep alive, and a captured launch holds its own).  A thread has eight neighbouring values, a warp the 256 of a block of codes, whose
 // largest value is one warp reduction.
 #include <cuda_bf16.h>
-#include <cuda_fp8.h>
+#include <cuda_fp16.h>
 
 #include <algorithm>
 #include <cmath>
@@ -18,7 +18,14 @@ namespace wkv6 {
 
 namespace {
 
-constexpr int kThreads = 256, kChunk = 4096, kPerThread = 8, kBlock = 256;
+#ifndef ADAMW_BLOCKS
+#define ADAMW_BLOCKS 2
+#endif
+#ifndef ADAMW_G
+#define ADAMW_G 2
+#endif
+constexpr int kThreads = 256, kPerThread = 8, kGroupValues = kThreads * kPerThread, kBlock = 256, kBlocksPerSm = ADAMW_BLOCKS;
+__host__ __device__ constexpr int groups(int bits) { return bits == 8 ? ADAMW_G : 1; }     // of eight values per thread and chunk
 
 struct Entry {
     void *p;
@@ -61,86 +68,163 @@ __host__ __device__ inline double power(double beta, int64_t t) {
     return r;
 }
 
-__device__ __forceinline__ float root(float x) {
+// Products and sums of the moments are rounded one by one, so that they have the bits of the formulas' elementary operations: a
+// moment in 8 bits that lies next to a border then never falls on its other side, and the scales of blocks do not drift apart from
+// those of another implementation.  (In pairs, mul.rn.f32x2 and add.rn.f32x2, ptxas contracts them into multiply-adds all the same,
+// and the moves that form the pairs cost what they save.)
+__device__ __forceinline__ float blend(float old, float keep, float add, float share) { return __fadd_rn(__fmul_rn(old, keep), __fmul_rn(add, share)); }
+
+__device__ __forceinline__ float reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float root_near(float x) {
     float y;
     asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
+// The square root rounded to nearest, for x >= 2^-100: Newton's step on the residual x - s^2, which a fused multiply-add gives
+// exactly (P. Markstein, IBM J. Res. Dev. 34, 1990).  Compared with sqrtf for all 2^24 values in [1, 4): no difference.
+__device__ __forceinline__ float root_exact(float x) {
+    float y;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    const float s = __fmul_rn(x, y);
+    return __fmaf_rn(__fmaf_rn(-s, s, x), __fmul_rn(y, 0.5f), s);
+}
+
+// Largest and smallest of three; a NaN among them stays.
+__device__ __forceinline__ float largest(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+__device__ __forceinline__ float smallest(float a, float b, float c) {
+    float y;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+using Eight = float[8];
+
+__device__ __forceinline__ float largest(const Eight &f) {
+    return largest(largest(f[0], f[1], f[2]), largest(f[3], f[4], f[5]), largest(f[6], f[7], f[7]));
+}
+
+__device__ __forceinline__ float smallest(const Eight &f) {
+    return smallest(smallest(f[0], f[1], f[2]), smallest(f[3], f[4], f[5]), smallest(f[6], f[7], f[7]));
+}
+
+// Eight neighbouring values as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, float (&f)[8]) {
-    if constexpr (sizeof(T) == 2) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+struct Raw {
+    uint4 w[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ Raw<T> load8(const T *p) {
+    Raw<T> r;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            f[2 * i] = __uint_as_float(w[i] << 16);
-            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    } else {
-        const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-        f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = reinterpret_cast<const uint4 *>(p)[i];
+    return r;
+}
+
+__device__ __forceinline__ void unpack(const Raw<__nv_bfloat16> &r, Eight &f) {
+    const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
 
-__device__ __forceinline__ void store8(float *p, const float (&f)[8]) {
+__device__ __forceinline__ void unpack(const Raw<float> &r, Eight &f) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        f[4 * i] = __uint_as_float(r.w[i].x);
+        f[4 * i + 1] = __uint_as_float(r.w[i].y);
+        f[4 * i + 2] = __uint_as_float(r.w[i].z);
+        f[4 * i + 3] = __uint_as_float(r.w[i].w);
+    }
+}
+
+__device__ __forceinline__ void store8(float *p, const Eight &f) {
     reinterpret_cast<float4 *>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
     reinterpret_cast<float4 *>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
 }
 
+// What eight values of a tensor need from memory.
+template <typename T, int BITS>
+struct Group {
+    Raw<T> p, g;
+    Raw<float> m, v;
+};
+template <typename T>
+struct Group<T, 8> {
+    Raw<T> p, g;
+    uint2 m, v;
+    float m_scale, v_scale;
+};
+
 __device__ __forceinline__ float value(float x) { return x; }
 __device__ __forceinline__ float value(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// fp32 to bf16: to nearest, or with 16 random bits added below the last kept one and then dropped.
-template <bool STOCHASTIC>
-__device__ __forceinline__ __nv_bfloat16 narrow(float x, uint32_t random) {
-    if (!STOCHASTIC || x != x) return __float2bfloat16_rn(x);       // the sum would carry a NaN into the sign
-    return __ushort_as_bfloat16((unsigned short)((__float_as_uint(x) + (random & 0xffffu)) >> 16));
-}
+// fp32 to bf16 (in the upper half of the word): 16 random bits are added below the last kept one, which carries into it with the
+// probability that keeps the mean.  x must not be a NaN: the sum would carry it into the sign.
+__device__ __forceinline__ uint32_t up_or_down(float x, uint32_t random) { return __float_as_uint(x) + ((random ^ (random >> 16)) & 0xffffu); }
 
-// q >= 0 in units of the block's scale onto the e4m3 grid, up or down by 16 random bits; never from above zero to zero, which would
-// divide the next update by eps alone.
-__device__ __forceinline__ float grid8(float q, uint32_t random) {
-    const float normal = __uint_as_float((__float_as_uint(q) + ((random >> 16) << 4)) & 0xfff00000u);
+// q >= 0 in units of the block's scale onto the e4m3 grid in the same way; never from above zero to zero, which would divide the next
+// update by eps alone.
+__device__ __forceinline__ float grid_normal(float q, uint32_t random) {
+    return __uint_as_float(((random >> 16) * 16u + __float_as_uint(q)) & 0xfff00000u);
+}
+__device__ __forceinline__ float grid_any(float q, uint32_t random) {
     const float tiny = fmaxf(floorf(fmaf(q, 512.f, (float)(random >> 16) * 0x1p-16f)), 1.f) * (1.f / 512.f);
-    return q >= 0x1p-6f ? normal : q > 0.f ? tiny : 0.f;
+    return q >= 0x1p-6f ? grid_normal(q, random) : q > 0.f ? tiny : 0.f;
 }
 
-__device__ __forceinline__ void decode8(uint64_t codes, float scale, float (&f)[8]) {
+__device__ __forceinline__ void decode8(uint2 codes, float scale, Eight &f) {
+    const uint32_t w[2] = {codes.x, codes.y};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes >> (16 * i)), __NV_E4M3);
-        const float2 x = __half22float2(__half2(h));
-        f[2 * i] = x.x * scale;
-        f[2 * i + 1] = x.y * scale;
+    for (int i = 0; i < 2; ++i) {
+        __half2 h[2];
+        uint32_t *u = reinterpret_cast<uint32_t *>(h);
+        asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(u[0]), "=r"(u[1]) : "r"(w[i]));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float2 x = __half22float2(h[j]);
+            f[4 * i + 2 * j] = __fmul_rn(x.x, scale);
+            f[4 * i + 2 * j + 1] = __fmul_rn(x.y, scale);
+        }
     }
 }
 
-__device__ __forceinline__ uint64_t encode8(const float (&f)[8]) {
-    uint64_t codes = 0;
+__device__ __forceinline__ uint2 encode8(const Eight &f) {
+    uint32_t w[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        codes |= (uint64_t)__nv_cvt_float2_to_fp8x2(make_float2(f[2 * i], f[2 * i + 1]), __NV_SATFINITE, __NV_E4M3) << (16 * i);
-    return codes;
+    for (int i = 0; i < 2; ++i)
+        asm("{\n.reg .b16 a, b;\ncvt.rn.satfinite.e4m3x2.f32 a, %2, %1;\ncvt.rn.satfinite.e4m3x2.f32 b, %4, %3;\nmov.b32 %0, {a, b};\n}"
+            : "=r"(w[i]) : "f"(f[4 * i]), "f"(f[4 * i + 1]), "f"(f[4 * i + 2]), "f"(f[4 * i + 3]));
+    return make_uint2(w[0], w[1]);
 }
 
 // Largest magnitude of the warp's 256 values, compared as bits: a NaN is larger than all others and stays.
-__device__ __forceinline__ float block_top(const float (&f)[8]) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-    return __uint_as_float(__reduce_max_sync(0xffffffffu, top));
+__device__ __forceinline__ float block_top(float top) {
+    return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu));
 }
 
 // A block's scale and the factor onto multiples of it.  Blocks below 2^-100 are zeros: their scale would leave the normal numbers.
 __device__ __forceinline__ float2 block_scale(float top) {
     if (top < 0x1p-100f) top = 0.f;
-    return make_float2(top * (1.f / 448.f), top > 0.f ? 448.f / top : 0.f);
+    return make_float2(top * (1.f / 448.f), top > 0.f ? __frcp_rn(top) * 448.f : 0.f);
 }
 
 template <typename T, int BITS, bool STOCHASTIC, int CAP>
-__global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ Table<CAP> a) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) adamw_kernel(const __grid_constant__ Table<CAP> a) {
+    constexpr int G = groups(BITS);
     __shared__ float shared[2];
     float step_size = a.step_size, inv_root2 = a.inv_root2;
     float decay = (float)(1.0 - a.lr * a.weight_decay);
@@ -158,120 +242,212 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constan
         decay = (float)(1.0 - lr * a.weight_decay);
     }
     const float b1 = (float)a.beta1, c1 = (float)(1.0 - a.beta1), b2 = (float)a.beta2, c2 = (float)(1.0 - a.beta2), eps = (float)a.eps;
-    const float gs = a.grad_scale != nullptr ? *a.grad_scale : 1.f;
+    const bool scaled = a.grad_scale != nullptr;
+    const float gs = scaled ? *a.grad_scale : 1.f;
     const uint32_t step_key = stir((uint32_t)t ^ a.seed_key);
     const int lane = threadIdx.x & 31;
-    for (uint32_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
-        int k = 0, end = a.count;
-        while (end - k > 1) {
-            const int mid = (k + end) >> 1;
-            if (a.e[mid].first_chunk <= chunk) k = mid; else end = mid;
-        }
-        const Entry &e = a.e[k];
-        const int64_t n = e.n, start = (int64_t)(chunk - e.first_chunk) * kChunk;
-        const uint32_t key = stir(e.index ^ step_key);
-        T *p = static_cast<T *>(e.p);
-        const T *g = static_cast<const T *>(e.g);
-        const bool aligned = ((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g)) & 15) == 0 &&
+
+    // a contiguous range of chunks: its first tensor by bisection, the next ones are the neighbours
+    uint32_t chunk = (uint32_t)((uint64_t)a.chunks * blockIdx.x / gridDim.x);
+    const uint32_t chunk_end = (uint32_t)((uint64_t)a.chunks * (blockIdx.x + 1) / gridDim.x);
+    int at = 0;
+    for (int bound = a.count; bound - at > 1;) {
+        const int mid = (at + bound) >> 1;
+        if (a.e[mid].first_chunk <= chunk) at = mid; else bound = mid;
+    }
+    // this thread's first value of a chunk; `whole`: the chunk can be moved as vectors
+    struct Place {
+        int k;
+        int64_t i;
+        bool whole;
+    };
+    auto locate = [&]() {
+        while (at + 1 < a.count && a.e[at + 1].first_chunk <= chunk) ++at;
+        const Entry &e = a.e[at];
+        const int64_t start = (int64_t)(chunk - e.first_chunk) * (G * kGroupValues);
+        const bool aligned = ((reinterpret_cast<uintptr_t>(e.p) | reinterpret_cast<uintptr_t>(e.g)) & 15) == 0 &&
                              ((reinterpret_cast<uintptr_t>(e.m) | reinterpret_cast<uintptr_t>(e.v)) & (BITS == 32 ? 15 : 7)) == 0;
+        return Place{at, start + threadIdx.x * kPerThread, aligned && start + G * kGroupValues <= e.n};
+    };
+    auto fetch = [&](const Entry &e, int64_t i, Group<T, BITS> &d) {
+        d.p = load8(static_cast<const T *>(e.p) + i);
+        d.g = load8(static_cast<const T *>(e.g) + i);
+        if constexpr (BITS == 32) {
+            d.m = load8(static_cast<const float *>(e.m) + i);
+            d.v = load8(static_cast<const float *>(e.v) + i);
+        } else {
+            d.m = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(e.m) + i);
+            d.v = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(e.v) + i);
+            d.m_scale = e.m_scale[(uint64_t)i / kBlock];
+            d.v_scale = e.v_scale[(uint64_t)i / kBlock];
+        }
+    };
+    // The step of eight values: x, m, v in, x, m and v (8 bits: codes) out; random: what rounds them (see stir()).
+    auto update = [&](const Entry &e, int64_t i, Eight &x, Eight &g, Eight &m, Eight &v, uint32_t (&random)[8], uint2 &mc, uint2 &vc) {
+        Eight r;
+        if (scaled) {
 #pragma unroll
-        for (int it = 0; it < kChunk / (kThreads * kPerThread); ++it) {
-            const int64_t i = start + it * (kThreads * kPerThread) + threadIdx.x * kPerThread;
-            const int64_t block = i / kBlock;                 // of this warp
-            if (i - lane * kPerThread >= n) break;            // the warp as a whole
-            const bool whole = aligned && i + kPerThread <= n;
-            const int have = i + kPerThread <= n ? kPerThread : i < n ? (int)(n - i) : 0;
-            float x[8], gr[8], m[8], v[8];
-            if (whole) {
-                load8(p + i, x);
-                load8(g + i, gr);
-                if constexpr (BITS == 32) {
-                    load8(static_cast<const float *>(e.m) + i, m);
-                    load8(static_cast<const float *>(e.v) + i, v);
-                } else {
-                    decode8(*reinterpret_cast<const uint64_t *>(static_cast<const uint8_t *>(e.m) + i), e.m_scale[block], m);
-                    decode8(*reinterpret_cast<const uint64_t *>(static_cast<const uint8_t *>(e.v) + i), e.v_scale[block], v);
-                }
-            } else {
-                uint64_t mc = 0, vc = 0;
+            for (int j = 0; j < 8; ++j) g[j] = __fmul_rn(g[j], gs);
+        }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const bool in = j < have;
-                    x[j] = in ? value(p[i + j]) : 0.f;
-                    gr[j] = in ? value(g[i + j]) : 0.f;
-                    if constexpr (BITS == 32) {
-                        m[j] = in ? static_cast<const float *>(e.m)[i + j] : 0.f;
-                        v[j] = in ? static_cast<const float *>(e.v)[i + j] : 0.f;
-                    } else if (in) {
-                        mc |= (uint64_t)static_cast<const uint8_t *>(e.m)[i + j] << (8 * j);
-                        vc |= (uint64_t)static_cast<const uint8_t *>(e.v)[i + j] << (8 * j);
-                    }
-                }
-                if constexpr (BITS == 8) {
-                    decode8(mc, e.m_scale[block], m);
-                    decode8(vc, e.v_scale[block], v);
-                }
-            }
-            const uint32_t high = (uint32_t)((uint64_t)i >> 32);
-            const uint32_t place = high ? stir(key + high) : key;      // eight neighbours share the upper word
-            uint32_t random[8];
-            float r[8];
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (BITS == 8) v[j] = __fmul_rn(v[j], v[j]);
+            m[j] = blend(m[j], b1, g[j], c1);
+            v[j] = blend(v[j], b2, __fmul_rn(g[j], g[j]), c2);
+            r[j] = BITS == 8 ? root_exact(v[j]) : root_near(v[j]);
+        }
+        if constexpr (STOCHASTIC || BITS == 8) {
+            // stir(i ^ key) but for its last step, which is left to each use; eight neighbours differ in three bits of the first word
+            const uint32_t high = (uint32_t)((uint64_t)i >> 32), key = stir(e.index ^ step_key);
+            uint32_t word = (uint32_t)i ^ (high ? stir(key + high) : key);
+            word ^= word >> 16;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if (STOCHASTIC || BITS == 8) random[j] = stir(((uint32_t)i + j) ^ place);
-                if constexpr (BITS == 8) v[j] *= v[j];
-                const float gj = gr[j] * gs;
-                m[j] = fmaf(gj, c1, m[j] * b1);
-                v[j] = fmaf(gj * gj, c2, v[j] * b2);
-                r[j] = root(v[j]);
-                x[j] = x[j] * decay - __fdividef(m[j] * step_size, fmaf(r[j], inv_root2, eps));
+                uint32_t w = (word ^ j) * 0x6A09E667u;
+                w ^= w >> 15;
+                random[j] = w * 0xBB67AE85u;
             }
-            uint64_t mc = 0, vc = 0;
-            if constexpr (BITS == 8) {
-                const float2 ms = block_scale(block_top(m)), vs = block_scale(block_top(r));
+        }
+        if constexpr (BITS == 8) {
+            const float2 ms = block_scale(block_top(largest(largest(m), -smallest(m), 0.f)));
+            float2 vs = block_scale(block_top(largest(r)));
+            Eight q;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    m[j] = ms.y > 0.f ? m[j] * ms.y : 0.f;
-                    r[j] = grid8(r[j] * vs.y, random[j]);
-                }
-                mc = encode8(m);
-                vc = encode8(r);
-                if (lane == 0) {
-                    e.m_scale[block] = ms.x;
-                    e.v_scale[block] = vs.x;
-                }
+            for (int j = 0; j < 8; ++j) q[j] = __fmul_rn(r[j], vs.y);
+            // Rare: a value whose code is below the normal ones (under 1 / 28672 of its block's largest), zeros, or roots of values under
+            // 2^-100.  One test for the warp; a NaN fails it.
+            if (__all_sync(0xffffffffu, smallest(q) >= 0x1p-6f && vs.x >= 0x1p-40f)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] = grid_normal(q[j], random[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) r[j] = __fsqrt_rn(v[j]);
+                vs = block_scale(block_top(largest(r)));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] = grid_any(__fmul_rn(r[j], vs.y), random[j]);
             }
-            if (whole) {
+            vc = encode8(q);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j] = __fmul_rn(m[j], ms.y);
+            mc = encode8(q);
+            if (lane == 0) {
+                e.m_scale[(uint64_t)i / kBlock] = ms.x;
+                e.v_scale[(uint64_t)i / kBlock] = vs.x;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = fmaf(m[j] * -step_size, reciprocal(fmaf(r[j], inv_root2, eps)), x[j] * decay);
+    };
+
+    // the next chunk's values travel while this one's are computed
+    Place next{};
+    Group<T, BITS> ahead[G];
+    auto advance = [&]() {
+        next = locate();
+        if (next.whole) {
+#pragma unroll
+            for (int u = 0; u < G; ++u) fetch(a.e[next.k], next.i + u * kGroupValues, ahead[u]);
+        }
+    };
+    if (chunk < chunk_end) advance();
+    while (chunk < chunk_end) {
+        const Place now = next;
+        Group<T, BITS> d[G];
+#pragma unroll
+        for (int u = 0; u < G; ++u) d[u] = ahead[u];
+        if (++chunk < chunk_end) advance();
+        const Entry &e = a.e[now.k];
+        if (now.whole) {
+#pragma unroll
+            for (int u = 0; u < G; ++u) {
+                const int64_t i = now.i + u * kGroupValues;
+                Eight x, g, m, v;
+                uint32_t random[8];
+                uint2 mc, vc;
+                unpack(d[u].p, x);
+                unpack(d[u].g, g);
+                if constexpr (BITS == 32) {
+                    unpack(d[u].m, m);
+                    unpack(d[u].v, v);
+                } else {
+                    decode8(d[u].m, d[u].m_scale, m);
+                    decode8(d[u].v, d[u].v_scale, v);
+                }
+                update(e, i, x, g, m, v, random, mc, vc);
                 if constexpr (sizeof(T) == 2) {
                     uint32_t w[4];
+                    const float most = largest(x);
+                    if (STOCHASTIC && most == most) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const __nv_bfloat162 h(narrow<STOCHASTIC>(x[2 * j], random[2 * j]), narrow<STOCHASTIC>(x[2 * j + 1], random[2 * j + 1]));
-                        w[j] = *reinterpret_cast<const uint32_t *>(&h);
+                        for (int j = 0; j < 4; ++j) w[j] = __byte_perm(up_or_down(x[2 * j], random[2 * j]), up_or_down(x[2 * j + 1], random[2 * j + 1]), 0x7632);
+                    } else {               // to nearest; or a NaN among the values
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+                            w[j] = *reinterpret_cast<const uint32_t *>(&h);
+                            if (STOCHASTIC) {
+                                if (x[2 * j] == x[2 * j]) w[j] = __byte_perm(up_or_down(x[2 * j], random[2 * j]), w[j], 0x7632);
+                                if (x[2 * j + 1] == x[2 * j + 1]) w[j] = __byte_perm(w[j], up_or_down(x[2 * j + 1], random[2 * j + 1]), 0x7610);
+                            }
+                        }
                     }
-                    *reinterpret_cast<uint4 *>(p + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4 *>(static_cast<T *>(e.p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
                 } else {
-                    store8(p + i, x);
+                    store8(static_cast<float *>(e.p) + i, x);
                 }
                 if constexpr (BITS == 32) {
                     store8(static_cast<float *>(e.m) + i, m);
                     store8(static_cast<float *>(e.v) + i, v);
                 } else {
-                    *reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(e.m) + i) = mc;
-                    *reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(e.v) + i) = vc;
+                    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(e.m) + i) = mc;
+                    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(e.v) + i) = vc;
                 }
-            } else {
+            }
+            continue;
+        }
+        // the end of a tensor, or one that does not start at a vector's boundary: value by value
+#pragma unroll 1
+        for (int u = 0; u < G; ++u) {
+            const int64_t i = now.i + u * kGroupValues, n = e.n;
+            if (i - lane * kPerThread >= n) break;             // the warp as a whole
+            const int have = i + kPerThread <= n ? kPerThread : i < n ? (int)(n - i) : 0;
+            T *p = static_cast<T *>(e.p);
+            const T *gp = static_cast<const T *>(e.g);
+            Eight x, g, m, v;
+            uint32_t random[8];
+            uint2 mc = make_uint2(0u, 0u), vc = make_uint2(0u, 0u);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (j < have) {
-                        if constexpr (sizeof(T) == 2) p[i + j] = narrow<STOCHASTIC>(x[j], random[j]); else p[i + j] = x[j];
-                        if constexpr (BITS == 32) {
-                            static_cast<float *>(e.m)[i + j] = m[j];
-                            static_cast<float *>(e.v)[i + j] = v[j];
-                        } else {
-                            static_cast<uint8_t *>(e.m)[i + j] = (uint8_t)(mc >> (8 * j));
-                            static_cast<uint8_t *>(e.v)[i + j] = (uint8_t)(vc >> (8 * j));
-                        }
+            for (int j = 0; j < 8; ++j) {
+                const bool in = j < have;
+                x[j] = in ? value(p[i + j]) : 0.f;
+                g[j] = in ? value(gp[i + j]) : 0.f;
+                if constexpr (BITS == 32) {
+                    m[j] = in ? static_cast<const float *>(e.m)[i + j] : 0.f;
+                    v[j] = in ? static_cast<const float *>(e.v)[i + j] : 0.f;
+                } else if (in) {
+                    (j < 4 ? mc.x : mc.y) |= (uint32_t)static_cast<const uint8_t *>(e.m)[i + j] << (8 * (j % 4));
+                    (j < 4 ? vc.x : vc.y) |= (uint32_t)static_cast<const uint8_t *>(e.v)[i + j] << (8 * (j % 4));
+                }
+            }
+            if constexpr (BITS == 8) {
+                decode8(mc, e.m_scale[(uint64_t)i / kBlock], m);
+                decode8(vc, e.v_scale[(uint64_t)i / kBlock], v);
+                __syncwarp();                                  // all have read the scales before one writes the new ones
+            }
+            update(e, i, x, g, m, v, random, mc, vc);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (j < have) {
+                    if constexpr (sizeof(T) == 2)
+                        p[i + j] = STOCHASTIC && x[j] == x[j] ? __ushort_as_bfloat16((unsigned short)(up_or_down(x[j], random[j]) >> 16)) : __float2bfloat16_rn(x[j]);
+                    else
+                        p[i + j] = x[j];
+                    if constexpr (BITS == 32) {
+                        static_cast<float *>(e.m)[i + j] = m[j];
+                        static_cast<float *>(e.v)[i + j] = v[j];
+                    } else {
+                        static_cast<uint8_t *>(e.m)[i + j] = (uint8_t)((j < 4 ? mc.x : mc.y) >> (8 * (j % 4)));
+                        static_cast<uint8_t *>(e.v)[i + j] = (uint8_t)((j < 4 ? vc.x : vc.y) >> (8 * (j % 4)));
                     }
                 }
             }
@@ -298,13 +474,14 @@ int launch(const wkv6_adamw &c, int64_t count, const wkv6_adamw_tensor *ts, cuda
     a.seed_key = stir((uint32_t)c.seed);
     a.step_size = (float)(c.lr / (1.0 - power(c.beta1, c.step)));
     a.inv_root2 = (float)(1.0 / sqrt(1.0 - power(c.beta2, c.step)));
+    constexpr int chunk_values = groups(BITS) * kGroupValues;
     int64_t i = 0;
     while (i < count) {
         a.count = 0;
         int64_t chunks = 0;
         for (; i < count && a.count < CAP; ++i) {
             if (ts[i].n == 0) continue;
-            const int64_t more = (ts[i].n + kChunk - 1) / kChunk;
+            const int64_t more = (ts[i].n + chunk_values - 1) / chunk_values;
             if (chunks + more > 0x7fffffffLL) {
                 if (a.count == 0) return fail(WKV6_ERR_UNSUPPORTED, "wkv6_adamw_step: tensor of %lld values", (long long)ts[i].n);
                 break;
@@ -314,7 +491,7 @@ int launch(const wkv6_adamw &c, int64_t count, const wkv6_adamw_tensor *ts, cuda
         }
         if (a.count == 0) break;
         a.chunks = (uint32_t)chunks;
-        const int64_t most = 4LL * sm_count();
+        const int64_t most = (int64_t)kBlocksPerSm * sm_count();
         adamw_kernel<T, BITS, STOCHASTIC, CAP><<<(unsigned)std::min(chunks, most), kThreads, 0, st>>>(a);
         const cudaError_t e = cudaGetLastError();
         if (e != cudaSuccess) return cuda_fail(e, "adamw_kernel launch");
