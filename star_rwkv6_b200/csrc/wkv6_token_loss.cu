@@ -1,14 +1,16 @@
 // Log-probabilities of given tokens under a model's logits, and the two losses that train on them: the clipped policy loss with a
-// KL term and the loss of paired log ratios.  For every token (row) with logits z[V], target a, temperature tau:
-//   c = max z,   s = sum_j exp((z_j - c) / tau),   lp = (z_a - c) / tau - log s,   p_j = exp((z_j - c) / tau) / s
+// KL term and the loss of paired log ratios.  For every token (row) with logits z[V], target a, temperature tau, k = log2(e) / tau:
+//   c = k max z,   s = sum_j 2^(k z_j - c),   lp = (k z_a - c - log2 s) ln 2,   p_j = 2^(k z_j - c) / s
 //   d lp / d z_j = (1[j = a] - p_j) / tau
-// Everything is bound by the bytes of the logits (65536 of them per token), so a row's maximum and sum are taken in one pass
-// (the sum is rescaled when the maximum grows), and where the gradient needs nothing but the row itself (policy loss) the row is
-// read again right behind that, out of the L2 cache (rows in flight: two 512-thread blocks per SM, 39 MB of bf16 rows of 65536).
+// Everything is bound by the bytes of the logits (65536 of them per token), and next by instructions: at the copy bandwidth a bf16
+// logit has to be done with in 11.  A row's maximum and sum are taken in one pass (the sum is rescaled when the maximum grows), and
+// where the gradient needs nothing but the row itself (policy loss) the row is gone through again right behind that, from its end to its
+// start: the end is still in shared memory, the rest in the L2 cache.
 // Rows that the mask leaves out, or whose target is no token, are not read: their log-probability and gradient are zero
 // whatever the logits hold.
-// The difference z - c is formed before it is scaled, so that it is exact near the maximum and does not overflow for logits at the
-// end of the type's range; a row of -inf has no distribution and gives NaN.
+// k z - c is one multiply-add: c is rounded, but it is the same c everywhere in a row, so that it cancels.  Logits near the end of the
+// type's range, where k z overflows, take a second way (`wide`): their maximum is subtracted before the scaling.  A row of -inf has no
+// distribution and gives NaN.
 // The reference has no trainer (its trainer files are empty); these operators stand beside the next-token loss.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -16,6 +18,8 @@
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
+#include <cstring>
+#include <type_traits>
 
 #include "wkv6_internal.h"
 
@@ -31,6 +35,7 @@ struct Rows {
     int T, V;
     float k;         // log2(e) / tau
     float inv_tau;
+    float low;       // logits of larger magnitude, as a row's maximum, take the wide way: -FLT_MAX / 4 / max(k, 1)
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -39,24 +44,12 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// (a + b) * c per component, two instructions for the pair
-__device__ __forceinline__ float2 add_mul(float2 a, float b, float c) {
-    unsigned long long x, y, w;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a.x), "f"(a.y));
-    asm("mov.b64 %0, {%1, %1};" : "=l"(y) : "f"(b));
-    asm("mov.b64 %0, {%1, %1};" : "=l"(w) : "f"(c));
-    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(y));
-    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(w));
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-    return r;
-}
-
 // Sixteen bytes of logits as fp32 pairs and back (each value rounded once, to nearest).
 template <typename T> struct Vec;
 
 template <> struct Vec<__nv_bfloat16> {
     static constexpr int N = 8;
+    static constexpr uint32_t kNone = 0xff80ff80u;      // -inf throughout
     static __device__ __forceinline__ void get(const uint4 &v, float2 (&f)[4]) {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -82,6 +75,7 @@ template <> struct Vec<__nv_bfloat16> {
 
 template <> struct Vec<__half> {
     static constexpr int N = 8;
+    static constexpr uint32_t kNone = 0xfc00fc00u;
     static __device__ __forceinline__ void get(const uint4 &v, float2 (&f)[4]) {
         const __half2 *p = reinterpret_cast<const __half2 *>(&v);
 #pragma unroll
@@ -107,6 +101,7 @@ template <> struct Vec<__half> {
 
 template <> struct Vec<float> {
     static constexpr int N = 4;
+    static constexpr uint32_t kNone = 0xff800000u;
     static __device__ __forceinline__ void get(const uint4 &v, float2 (&f)[2]) {
         f[0] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
         f[1] = make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
@@ -128,79 +123,217 @@ __device__ __forceinline__ int head_of(const T *p, int n) {
     return h < n ? h : n;
 }
 
-// (maximum, sum of exp2((z - maximum) k)) of two parts of a row; the same bits whichever part comes first, so that all lanes of an
-// exchange end with one result
-__device__ __forceinline__ void merge(float &mx, float &sum, float mx2, float sum2, float k) {
-    const float m = fmaxf(mx, mx2);
-    sum = __fadd_rn(__fmul_rn(sum, ex2((mx - m) * k)), __fmul_rn(sum2, ex2((mx2 - m) * k)));
-    mx = m;
+__device__ __forceinline__ float warp_max(float x) {
+    float y;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-// This thread's share (every THREADS-th vector) of a row.  The maximum starts at the lowest finite value and not at -inf: a part
-// that holds nothing but -inf then adds zeros.
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+
+// What a part of a row has come to: its maximum (not below Rows::low, so that parts of nothing but -inf add zeros), c = k max, and the sum.
+struct Part {
+    float mx, c, sum;
+};
+
+// Takes U vectors into a part.
+template <typename T, int U>
+__device__ __forceinline__ void take(const uint4 (&q)[U], float k, Part &r) {
+    constexpr int N = Vec<T>::N;
+    float m = r.mx;
+#pragma unroll
+    for (int u = 0; u < U; ++u) m = fmaxf(m, Vec<T>::max(q[u]));
+    const float c = m * k;
+    float sum0 = r.sum * ex2(r.c - c), sum1 = 0.f;
+    r.mx = m;
+    r.c = c;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float2 f[N / 2];
+        Vec<T>::get(q[u], f);
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) {
+            sum0 += ex2(fmaf(f[e].x, k, -c));
+            sum1 += ex2(fmaf(f[e].y, k, -c));
+        }
+    }
+    r.sum = sum0 + sum1;
+}
+
+// g (1[j = a] - p_j) of a vector of logits: neg = -g / sum, `at` = a's place in the vector.  (Products and sums are kept apart, so that all
+// kernels that come here give the same bits.)  WIDE: c is the maximum itself.
+template <typename T, bool WIDE>
+__device__ __forceinline__ float gradient_of(float z, float k, float c, float neg) {
+    return __fmul_rn(ex2(WIDE ? (z - c) * k : fmaf(z, k, -c)), neg);
+}
+template <typename T, bool WIDE>
+__device__ __forceinline__ uint4 gradient_of(const uint4 &q, int at, float k, float c, float neg, float g) {
+    constexpr int N = Vec<T>::N;
+    float2 f[N / 2];
+    Vec<T>::get(q, f);
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) f[e] = make_float2(gradient_of<T, WIDE>(f[e].x, k, c, neg), gradient_of<T, WIDE>(f[e].y, k, c, neg));
+    if (at >= 0) {
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) {
+            if (at == 2 * e) f[e].x = __fadd_rn(f[e].x, g);
+            if (at == 2 * e + 1) f[e].y = __fadd_rn(f[e].y, g);
+        }
+    }
+    return Vec<T>::put(f);
+}
+
+// A row's vectors, and its values outside them: fewer than two vectors' worth, in front (head) and behind (from tail on).
+struct Cut {
+    int head, vecs, tail, loose;
+    __device__ __forceinline__ int at(int i) const { return i < head ? i : tail + i - head; }
+};
+template <typename T>
+__device__ __forceinline__ Cut cut_of(const T *p, int V) {
+    Cut l;
+    l.head = head_of(p, V);
+    l.vecs = (V - l.head) / Vec<T>::N;
+    l.tail = l.head + l.vecs * Vec<T>::N;
+    l.loose = l.head + V - l.tail;
+    return l;
+}
+
+template <typename T>
+__device__ __forceinline__ void take_loose(const T *z, const Cut &l, int first, int step, float k, Part &r) {
+    for (int i = first; i < l.loose; i += step) {
+        const float x = Vec<T>::get1(z[l.at(i)]), m = fmaxf(r.mx, x), c = m * k;
+        r.sum = r.sum * ex2(r.c - c) + ex2(fmaf(x, k, -c));
+        r.mx = m;
+        r.c = c;
+    }
+}
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void gradient_loose(const T *z, T *out, const Cut &l, int target, float k, float c, float neg, float g, int first, int step) {
+    for (int i = first; i < l.loose; i += step) {
+        const int j = l.at(i);
+        float x = gradient_of<T, WIDE>(Vec<T>::get1(z[j]), k, c, neg);
+        if (j == target) x = __fadd_rn(x, g);
+        out[j] = Vec<T>::one(x);
+    }
+}
+
+#ifndef TL_U
+#define TL_U 4
+#endif
+constexpr int kU = TL_U;         // vectors that a thread requests at once, while it computes on as many
+
+// Logits that are read once leave no line in the first-level cache; KEEP (the row will be read again): nor do the others, but with that
+// hint they also leave the second-level cache early (policy loss at 8192 x 65536: 340 MB read per 198 MB of rows, and 450 us for 392).
+template <bool KEEP>
+__device__ __forceinline__ uint4 load16(const uint4 *p) {
+    if (KEEP) return __ldg(p);
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// A thread's vectors of a row (v[0], v[THREADS], ...), kU at a time.
 template <typename T, int THREADS>
-__device__ __forceinline__ void row_part(const T *z, int V, int tid, float k, float &mx, float &sum) {
-    constexpr int N = Vec<T>::N, U = 4;
-    mx = -FLT_MAX;
-    sum = 0.f;
-    const int head = head_of(z, V), vecs = (V - head) / N;
-    const uint4 *v = reinterpret_cast<const uint4 *>(z + head);
-    for (int i0 = tid; i0 < vecs; i0 += THREADS * U) {
-        uint4 q[U];
-        float m = mx;
+struct Share {
+    const uint4 *v;
+    int count;
+    __device__ __forceinline__ Share(const uint4 *vectors, int n, int tid) : v(vectors + tid), count((n - tid + THREADS - 1) / THREADS) {}
+    __device__ __forceinline__ int batches() const { return (count + kU - 1) / kU; }
+    // Vectors that do not exist come as -inf, which adds nothing.
+    template <bool KEEP>
+    __device__ __forceinline__ void load(int b, uint4 (&q)[kU]) const {
+        const uint4 *p = v + (int64_t)b * (kU * THREADS);
+        if ((b + 1) * kU <= count) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i0 + u * THREADS < vecs) q[u] = __ldg(v + i0 + u * THREADS);
+            for (int u = 0; u < kU; ++u) q[u] = load16<KEEP>(p + u * THREADS);
+        } else {
+            const uint32_t none = Vec<T>::kNone;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i0 + u * THREADS < vecs) m = fmaxf(m, Vec<T>::max(q[u]));
-        sum *= ex2((mx - m) * k);
-        mx = m;
-        float2 s2 = make_float2(0.f, 0.f);
+            for (int u = 0; u < kU; ++u) q[u] = b * kU + u < count ? load16<KEEP>(p + u * THREADS) : make_uint4(none, none, none, none);
+        }
+    }
+};
+
+// Two batches of a share: one is computed on while the other one travels.
+struct Batches {
+    uint4 even[kU], odd[kU];
+};
+
+// Maximum and sum over a thread's share of a row.  The last batch stays in x.odd, the one before it in x.even.
+template <typename T, int THREADS, bool KEEP>
+__device__ __forceinline__ void row_part(const Share<T, THREADS> &w, float k, Part &r, Batches &x) {
+    const int n = w.batches();
+    int b = n & 1;
+    if (b) w.template load<KEEP>(0, x.odd);
+    if (n > b) w.template load<KEEP>(b, x.even);
+    if (b) take<T, kU>(x.odd, k, r);
+    for (; b < n; b += 2) {
+        w.template load<KEEP>(b + 1, x.odd);
+        take<T, kU>(x.even, k, r);
+        if (b + 2 < n) w.template load<KEEP>(b + 2, x.even);
+        take<T, kU>(x.odd, k, r);
+    }
+}
+
+// What row_part leaves, for a gradient that has no sum in front of it.
+template <typename T, int THREADS>
+__device__ __forceinline__ void last_batches(const Share<T, THREADS> &w, Batches &x) {
+    const int n = w.batches();
+    if (n > 0) w.template load<false>(n - 1, x.odd);
+    if (n > 1) w.template load<false>(n - 2, x.even);
+}
+
+// The gradient over a thread's share of a row, into out[0], out[THREADS], ..., from the end to the start: the end is in registers, what is
+// before it was read last.  own = the number of the thread's vector that holds the target (at place `at`), or -1.  STREAM: the gradient
+// is not to displace rows that are waiting for theirs in the second-level cache (387 us instead of 374 otherwise).
+template <typename T, int THREADS, bool STREAM>
+__device__ __forceinline__ void row_gradient(const Share<T, THREADS> &w, Batches &x, uint4 *out, int own, int at, float k, float c, float neg, float g) {
+    auto put = [&](int b, const uint4 (&q)[kU]) {
+        uint4 *p = out + (int64_t)b * (kU * THREADS);
+        const bool whole = (b + 1) * kU <= w.count;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i0 + u * THREADS < vecs) {
-                float2 f[N / 2];
-                Vec<T>::get(q[u], f);
-#pragma unroll
-                for (int e = 0; e < N / 2; ++e) {
-                    const float2 d = add_mul(f[e], -mx, k);
-                    s2.x += ex2(d.x);
-                    s2.y += ex2(d.y);
-                }
+        for (int u = 0; u < kU; ++u) {
+            if (whole || b * kU + u < w.count) {
+                const uint4 y = gradient_of<T, false>(q[u], b * kU + u == own ? at : -1, k, c, neg, g);
+                if (STREAM) __stcs(p + u * THREADS, y);
+                else p[u * THREADS] = y;
             }
         }
-        sum += s2.x + s2.y;
+    };
+    int b = w.batches() - 1;
+    for (; b >= 1; b -= 2) {
+        put(b, x.odd);
+        if (b >= 2) w.template load<false>(b - 2, x.odd);
+        put(b - 1, x.even);
+        if (b >= 3) w.template load<false>(b - 3, x.even);
     }
-    const int tail = head + vecs * N, loose = head + V - tail;      // values outside the vectors: fewer than two vectors' worth
-    for (int i = tid; i < loose; i += THREADS) {
-        const float x = Vec<T>::get1(z[i < head ? i : tail + i - head]), m = fmaxf(mx, x);
-        sum = sum * ex2((mx - m) * k) + ex2((x - m) * k);
-        mx = m;
-    }
+    if (b == 0) put(0, x.odd);
 }
 
-// g_j = c (1[j = a] - p_j) over the vectors of the gradient row from `first` on, every `step`-th.  The logits' row may lie at
-// another offset from the 16-byte boundaries than the gradient's: its values are then loaded one by one.  (Products and sums are
-// kept apart, so that both kernels that come here give the same bits.)
-template <typename T>
-__device__ __forceinline__ void row_gradient(const T *z, T *g, int V, int target, float mx, float inv_sum, float k, float c, int first, int step) {
+// The same without shared memory: for rows of a few KB, for the wide way, and for logits that lie at another offset from the 16-byte
+// boundaries than the gradient (their values are loaded one by one).
+template <typename T, bool WIDE>
+__device__ __forceinline__ void row_gradient_direct(const T *z, T *out, const Cut &l, int target, float k, float c, float neg, float g, int first, int step) {
     constexpr int N = Vec<T>::N, U = 2;
-    const int head = head_of(g, V), vecs = (V - head) / N;
-    const bool same = head_of(z, V) == head;
-    const float neg = -c * inv_sum;
-    for (int i0 = first; i0 < vecs; i0 += step * U) {
+    const bool same = (reinterpret_cast<uintptr_t>(z) - reinterpret_cast<uintptr_t>(out)) % 16 == 0;
+    const int at = target - l.head, own = at < 0 ? -1 : at / N;
+    for (int i0 = first; i0 < l.vecs; i0 += step * U) {
         uint4 q[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * step;
-            if (i < vecs) {
+            if (i < l.vecs) {
                 if (same) {
-                    q[u] = __ldg(reinterpret_cast<const uint4 *>(z + head) + i);
+                    q[u] = __ldg(reinterpret_cast<const uint4 *>(z + l.head) + i);
                 } else {
                     T x[N];
 #pragma unroll
-                    for (int e = 0; e < N; ++e) x[e] = z[head + (int64_t)i * N + e];
+                    for (int e = 0; e < N; ++e) x[e] = z[l.head + (int64_t)i * N + e];
                     memcpy(&q[u], x, 16);
                 }
             }
@@ -208,46 +341,51 @@ __device__ __forceinline__ void row_gradient(const T *z, T *g, int V, int target
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u * step;
-            if (i < vecs) {
-                float2 f[N / 2];
-                Vec<T>::get(q[u], f);
-#pragma unroll
-                for (int e = 0; e < N / 2; ++e) {
-                    const float2 d = add_mul(f[e], -mx, k);
-                    f[e] = make_float2(__fmul_rn(ex2(d.x), neg), __fmul_rn(ex2(d.y), neg));
-                }
-                const int at = target - head - i * N;
-                if (at >= 0 && at < N) {
-#pragma unroll
-                    for (int e = 0; e < N / 2; ++e) {
-                        if (at == 2 * e) f[e].x = __fadd_rn(f[e].x, c);
-                        if (at == 2 * e + 1) f[e].y = __fadd_rn(f[e].y, c);
-                    }
-                }
-                reinterpret_cast<uint4 *>(g + head)[i] = Vec<T>::put(f);
-            }
+            if (i < l.vecs) reinterpret_cast<uint4 *>(out + l.head)[i] = gradient_of<T, WIDE>(q[u], i == own ? at % N : -1, k, c, neg, g);
         }
     }
-    const int tail = head + vecs * N, loose = head + V - tail;
-    for (int i = first; i < loose; i += step) {
-        const int j = i < head ? i : tail + i - head;
-        float x = __fmul_rn(ex2((Vec<T>::get1(z[j]) - mx) * k), neg);
-        if (j == target) x = __fadd_rn(x, c);
-        g[j] = Vec<T>::one(x);
+    gradient_loose<T, WIDE>(z, out, l, target, k, c, neg, g, first, step);
+}
+
+// Maximum and sum of 2^((z - maximum) k) over a thread's part of a row that takes the wide way.
+template <typename T>
+__device__ __forceinline__ void row_part_wide(const T *z, int V, int first, int step, float k, float &mx, float &sum) {
+    mx = -FLT_MAX;
+    sum = 0.f;
+    for (int i = first; i < V; i += step) {
+        const float x = Vec<T>::get1(z[i]), m = fmaxf(mx, x);
+        sum = sum * ex2((mx - m) * k) + ex2((x - m) * k);
+        mx = m;
+    }
+}
+
+// (c, sum) of a row from those of its threads, whose sums are of powers 2^(... - k c).  Every thread gets the same bits.
+template <int THREADS, int TURN>
+__device__ __forceinline__ void gather(float &c, float &sum, float k) {
+    const float m = warp_max(c);
+    sum = warp_sum(sum * ex2((c - m) * k));
+    c = m;
+    if constexpr (THREADS != 32) {
+        __shared__ float2 part[THREADS / 32];
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) part[threadIdx.x >> 5] = make_float2(c, sum);
+        __syncthreads();
+        const float2 p = lane < THREADS / 32 ? part[lane] : make_float2(c, 0.f);
+        c = warp_max(p.x);
+        sum = warp_sum(p.y * ex2((p.x - c) * k));
     }
 }
 
 template <typename T>
-__device__ __forceinline__ void row_zero(T *g, int V, int first, int step) {
-    constexpr int N = Vec<T>::N;
-    const int head = head_of(g, V), vecs = (V - head) / N, tail = head + vecs * N, loose = head + V - tail;
-    for (int i = first; i < vecs; i += step) reinterpret_cast<uint4 *>(g + head)[i] = make_uint4(0u, 0u, 0u, 0u);
-    for (int i = first; i < loose; i += step) g[i < head ? i : tail + i - head] = Vec<T>::one(0.f);
+__device__ __forceinline__ void row_zero(T *g, const Cut &l, int first, int step) {
+    for (int i = first; i < l.vecs; i += step) reinterpret_cast<uint4 *>(g + l.head)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = first; i < l.loose; i += step) g[l.at(i)] = Vec<T>::one(0.f);
 }
 
 template <typename T>
 __device__ __forceinline__ const T *row_of(const Rows &a, int64_t row) {
-    return static_cast<const T *>(a.z) + (row / a.T) * a.seq_stride + (row % a.T) * a.row_stride;
+    const uint32_t s = (uint32_t)row / (uint32_t)a.T, t = (uint32_t)row - s * (uint32_t)a.T;      // there are fewer than 2^31 rows
+    return static_cast<const T *>(a.z) + s * a.seq_stride + t * a.row_stride;
 }
 
 // The row's target, or -1 where the row does not count.
@@ -269,16 +407,16 @@ struct Policy {
 };
 
 constexpr int kCountRows = 1024;    // rows of a part where tokens are counted over all sequences
-constexpr int kRowThreads = 512, kWarpRows = 8;
+constexpr int kWarpRows = 8;
 
-// The last block to finish adds up the rows, in an order that does not depend on which block that is.
-__device__ __forceinline__ void total_loss(const Policy &q, int64_t rows) {
+// The last block to draw a number behind its rows' losses adds up all rows, in an order that does not depend on which block that is.
+// Thread 0 draws it while the gradient is still to be written.
+__device__ __forceinline__ void draw_number(const Policy &q, bool &last) {
+    __threadfence();
+    last = atomicAdd(q.done, 1u) == gridDim.x - 1;
+}
+__device__ __forceinline__ void total_loss(const Policy &q, int64_t rows, const bool &last) {
     __shared__ double part[32];
-    __shared__ bool last;
-    if (threadIdx.x == 0) {
-        __threadfence();
-        last = atomicAdd(q.done, 1u) == gridDim.x - 1;
-    }
     __syncthreads();
     if (!last) return;
     __threadfence();
@@ -294,98 +432,127 @@ __device__ __forceinline__ void total_loss(const Policy &q, int64_t rows) {
     }
 }
 
-// THREADS = 512: a block per row; 32: a warp per row (rows of a few KB, where a block's reduction would cost more than its row).
-// POLICY: the loss and, with g, the gradient behind the log-probabilities.
+#ifndef TL_THREADS
+#define TL_THREADS 256
+#endif
+constexpr int kRowThreads = TL_THREADS;     // of a long row
+__host__ __device__ constexpr int row_blocks(int threads) { return 1024 / (threads == 32 ? 32 * kWarpRows : threads); }   // per SM
+
+// What a row's loss takes beside its log-probability, requested before the row.
+struct Terms {
+    float adv = 0.f, old = 0.f, ref = 0.f;
+    int n = 0;
+};
+__device__ __forceinline__ Terms terms_of(const Rows &a, const Policy &q, int64_t row) {
+    Terms t;
+    t.adv = q.advantages[row];
+    t.old = q.old_lp[row];
+    if (q.ref_lp != nullptr) t.ref = q.ref_lp[row];
+    if (q.reduction == WKV6_MEAN)
+        for (int i = threadIdx.x & 31; i < q.parts; i += 32) t.n += q.counts[i];
+    else if (q.reduction == WKV6_SEQUENCE_MEAN)
+        t.n = q.counts[(uint32_t)row / (uint32_t)a.T];
+    return t;
+}
+
+// Loss of a row and its derivative by the row's log-probability.
+__device__ __forceinline__ float2 loss_of(const Rows &a, const Policy &q, Terms t, float lp) {
+    float w = q.scale;
+    if (q.reduction == WKV6_MEAN) {
+        t.n = __reduce_add_sync(0xffffffffu, t.n);
+        w = q.scale / (float)t.n;
+    } else if (q.reduction == WKV6_SEQUENCE_MEAN) {
+        w = q.scale / ((float)t.n * (float)((uint32_t)a.rows / (uint32_t)a.T));
+    }
+    // comparisons written so that a NaN ratio is not clipped away
+    const float rho = expf(lp - t.old), free = rho * t.adv;
+    const float clipped = (rho < q.low ? q.low : rho > q.high ? q.high : rho) * t.adv;
+    const bool open = !(free > clipped);
+    float loss = open ? -free : -clipped, slope = open ? -free : 0.f;
+    if (q.ref_lp != nullptr) {     // exp(d) - d - 1 is d^2 / 2 for small d: taken from exp(d) - 1
+        const float d = t.ref - lp, e = expm1f(d);
+        loss += q.kl * (e - d);
+        slope -= q.kl * e;
+    }
+    return make_float2(loss * w, slope * w);
+}
+
+// From the threads' parts of a row to its log-probability: r becomes the row's (c and sum), `wide` says how.
+template <typename T, int THREADS>
+__device__ __forceinline__ float finish_row(const Rows &a, const T *z, float zt, int tid, Part &r, bool &wide) {
+    gather<THREADS, 0>(r.c, r.sum, 1.f);
+    const float end = -a.low * a.k;      // the same in all threads; a NaN in the sum stays what it is
+    wide = !(r.c > -end && r.c < end);
+    if (wide) {
+        row_part_wide(z, a.V, tid, THREADS, a.k, r.c, r.sum);
+        gather<THREADS, 1>(r.c, r.sum, a.k);
+        return (zt - r.c) * a.inv_tau - logf(r.sum);
+    }
+    return (fmaf(zt, a.k, -r.c) - log2f(r.sum)) * 0.69314718055994531f;
+}
+
+// THREADS = 32: a warp per row, several to a block (rows of a few KB, where a block's reduction would cost more than its row);
+// otherwise a block per row.  POLICY: the loss and, with g, the gradient behind the log-probabilities.
 template <typename T, int THREADS, bool POLICY>
-__global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, THREADS == 32 ? 4 : 2)
+__global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, row_blocks(THREADS))
 token_rows_kernel(const Rows a, float *__restrict__ lp_out, float2 *__restrict__ stat, const Policy q, float *__restrict__ coefficient,
                   T *__restrict__ g) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = THREADS == 32 ? lane : threadIdx.x;
-    const int64_t row = THREADS == 32 ? (int64_t)blockIdx.x * kWarpRows + warp : blockIdx.x;
+    __shared__ bool last;
+    const int tid = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x;
+    const int64_t row = THREADS == 32 ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
     if (THREADS != 32 || row < a.rows) {
         const int target = target_of(a, row);
-        float lp = 0.f, c = 0.f, loss = 0.f, mx = 0.f, inv_sum = 0.f;
         const T *z = row_of<T>(a, row);
+        const Cut l = cut_of(z, a.V);
+        const Share<T, THREADS> share(reinterpret_cast<const uint4 *>(z + l.head), l.vecs, tid);
+        float lp = 0.f, inv_sum = 0.f;
+        float2 loss = make_float2(0.f, 0.f);
+        Part r{a.low, a.low * a.k, 0.f};
+        bool wide = false;
+        Batches x;
         if (target >= 0) {
-            float adv = 0.f, old = 0.f, ref = 0.f;
-            int n = 0;
-            if constexpr (POLICY) {       // requested before the row
-                adv = q.advantages[row];
-                old = q.old_lp[row];
-                if (q.ref_lp != nullptr) ref = q.ref_lp[row];
-                if (q.reduction == WKV6_MEAN)
-                    for (int i = lane; i < q.parts; i += 32) n += q.counts[i];
-                else if (q.reduction == WKV6_SEQUENCE_MEAN)
-                    n = q.counts[row / a.T];
-            }
-            float sum;
+            Terms t;
+            if constexpr (POLICY) t = terms_of(a, q, row);
             const float zt = Vec<T>::get1(z[target]);
-            row_part<T, THREADS>(z, a.V, tid, a.k, mx, sum);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const float m2 = __shfl_xor_sync(0xffffffffu, mx, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
-                merge(mx, sum, m2, s2, a.k);
-            }
-            if constexpr (THREADS != 32) {
-                __shared__ float2 part[THREADS / 32];
-                if (lane == 0) part[warp] = make_float2(mx, sum);
-                __syncthreads();
-                const float2 p = part[lane % (THREADS / 32)];
-                mx = p.x;
-                sum = p.y;
-#pragma unroll
-                for (int o = THREADS / 64; o > 0; o >>= 1) {
-                    const float m2 = __shfl_xor_sync(0xffffffffu, mx, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
-                    merge(mx, sum, m2, s2, a.k);
-                }
-            }
-            inv_sum = 1.f / sum;
-            lp = (zt - mx) * a.inv_tau - logf(sum);
-            if constexpr (POLICY) {
-                float w = q.scale;
-                if (q.reduction == WKV6_MEAN) {
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-                    w = q.scale / (float)n;
-                } else if (q.reduction == WKV6_SEQUENCE_MEAN) {
-                    w = q.scale / ((float)n * (float)(a.rows / a.T));
-                }
-                // comparisons written so that a NaN ratio is not clipped away
-                const float rho = expf(lp - old), free = rho * adv;
-                const float clipped = (rho < q.low ? q.low : rho > q.high ? q.high : rho) * adv;
-                const bool open = !(free > clipped);
-                loss = open ? -free : -clipped;
-                c = open ? -free : 0.f;
-                if (q.ref_lp != nullptr) {     // exp(d) - d - 1 is d^2 / 2 for small d: taken from exp(d) - 1
-                    const float d = ref - lp, e = expm1f(d);
-                    loss += q.kl * (e - d);
-                    c -= q.kl * e;
-                }
-                loss *= w;
-                c *= w;
-            }
+            row_part<T, THREADS, POLICY>(share, a.k, r, x);
+            take_loose(z, l, tid, THREADS, a.k, r);
+            lp = finish_row<T, THREADS>(a, z, zt, tid, r, wide);
+            inv_sum = 1.f / r.sum;
+            if constexpr (POLICY) loss = loss_of(a, q, t, lp);
         }
         if (tid == 0) {
             lp_out[row] = lp;
-            if (stat != nullptr) stat[row] = make_float2(mx, inv_sum);
+            if (stat != nullptr) stat[row] = make_float2(r.c, wide ? -inv_sum : inv_sum);
             if constexpr (POLICY) {
-                q.row_loss[row] = loss;
-                coefficient[row] = c;
+                q.row_loss[row] = loss.x;
+                coefficient[row] = loss.y;
+                if (THREADS != 32) draw_number(q, last);
             }
         }
         if constexpr (POLICY) {
             if (g != nullptr) {
                 T *gr = g + row * a.V;
-                if (c != 0.f)                  // NaN included
-                    row_gradient(z, gr, a.V, target, mx, inv_sum, a.k, c * a.inv_tau, tid, THREADS);
-                else
-                    row_zero(gr, a.V, tid, THREADS);
+                const float gc = loss.y * a.inv_tau, neg = -gc * inv_sum;
+                if (loss.y == 0.f) {                 // a NaN is not
+                    row_zero(gr, cut_of(gr, a.V), tid, THREADS);
+                } else if (wide) {
+                    row_gradient_direct<T, true>(z, gr, cut_of(gr, a.V), target, a.k, r.c, neg, gc, tid, THREADS);
+                } else if ((reinterpret_cast<uintptr_t>(z) - reinterpret_cast<uintptr_t>(gr)) % 16 == 0) {
+                    const int at = target - l.head, vec = at / Vec<T>::N, own = at >= 0 && vec % THREADS == tid ? vec / THREADS : -1;
+                    row_gradient<T, THREADS, true>(share, x, reinterpret_cast<uint4 *>(gr + l.head) + tid, own, at % Vec<T>::N, a.k, r.c, neg, gc);
+                    gradient_loose<T, false>(z, gr, l, target, a.k, r.c, neg, gc, tid, THREADS);
+                } else {
+                    row_gradient_direct<T, false>(z, gr, cut_of(gr, a.V), target, a.k, r.c, neg, gc, tid, THREADS);
+                }
             }
         }
     }
     if constexpr (POLICY) {
-        if (THREADS == 32) __syncthreads();
-        total_loss(q, a.rows);
+        if (THREADS == 32) {
+            __syncthreads();
+            if (threadIdx.x == 0) draw_number(q, last);
+        }
+        total_loss(q, a.rows, last);
     }
 }
 
@@ -394,22 +561,39 @@ token_rows_kernel(const Rows a, float *__restrict__ lp_out, float2 *__restrict__
 // A block takes a part of a row (blockIdx.y), so that few long rows fill the GPU too.  `unless_one`: nothing is done where *factor
 // is 1 (the gradient is there already).
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, THREADS == 32 ? 4 : 3)
+__global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, row_blocks(THREADS))
 token_gradient_kernel(const Rows a, const float2 *__restrict__ stat, const float *__restrict__ coefficient, int per_sequence,
                       const float *__restrict__ factor, int unless_one, T *__restrict__ g) {
     const float f = factor != nullptr ? *factor : 1.f;
     if (unless_one && f == 1.f) return;
     const int64_t row = THREADS == 32 ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= a.rows) return;
-    const int first = THREADS == 32 ? threadIdx.x & 31 : blockIdx.y * THREADS + threadIdx.x, step = THREADS == 32 ? 32 : THREADS * gridDim.y;
+    const int tid = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x, first = blockIdx.y * THREADS + tid, step = THREADS * gridDim.y;
     const int target = target_of(a, row);
-    const float c = target < 0 ? 0.f : coefficient[per_sequence ? row / a.T : row] * f * a.inv_tau;
+    const float gc = target < 0 ? 0.f : coefficient[per_sequence ? (uint32_t)row / (uint32_t)a.T : row] * f * a.inv_tau;
+    const T *z = row_of<T>(a, row);
     T *gr = g + row * a.V;
-    if (c != 0.f) {
-        const float2 s = stat[row];
-        row_gradient(row_of<T>(a, row), gr, a.V, target, s.x, s.y, a.k, c, first, step);
+    const Cut l = cut_of(gr, a.V);
+    if (gc == 0.f) {
+        row_zero(gr, l, first, step);
+        return;
+    }
+    const float2 s = stat[row];
+    if (signbit(s.y)) {
+        row_gradient_direct<T, true>(z, gr, l, target, a.k, s.x, gc * s.y, gc, first, step);
+    } else if ((reinterpret_cast<uintptr_t>(z) - reinterpret_cast<uintptr_t>(gr)) % 16 == 0) {
+        const int each = (l.vecs + gridDim.y - 1) / gridDim.y, begin = each * blockIdx.y, n = min(each, l.vecs - begin);
+        if (n > 0) {
+            const int at = target - l.head, vec = at / Vec<T>::N - begin;
+            const int own = at >= 0 && vec >= 0 && vec < n && vec % THREADS == tid ? vec / THREADS : -1;
+            const Share<T, THREADS> share(reinterpret_cast<const uint4 *>(z + l.head) + begin, n, tid);
+            Batches x;
+            last_batches(share, x);
+            row_gradient<T, THREADS, false>(share, x, reinterpret_cast<uint4 *>(gr + l.head) + begin + tid, own, at % Vec<T>::N, a.k, s.x, -gc * s.y, gc);
+        }
+        gradient_loose<T, false>(z, gr, l, target, a.k, s.x, -gc * s.y, gc, first, step);
     } else {
-        row_zero(gr, a.V, first, step);
+        row_gradient_direct<T, false>(z, gr, l, target, a.k, s.x, -gc * s.y, gc, first, step);
     }
 }
 
@@ -492,8 +676,25 @@ __global__ void __launch_bounds__(256) preference_pairs_kernel(int pairs, const 
     }
 }
 
-// A warp per row up to this many bytes of logits, a block above.
-constexpr int64_t kWarpRowBytes = 4096;
+// Threads of a row by the bytes of its logits: a warp up to 4 KB, 128 up to 32 KB, kRowThreads above, so that each has several vectors.
+int row_threads(const wkv6_token_logits *p) {
+    const int64_t n = (int64_t)p->V * (int64_t)dtype_size(p->dtype);
+    return n <= 4096 ? 32 : n <= 32768 ? 128 : kRowThreads;
+}
+
+// f(std::integral_constant<int, THREADS>, T *) for the call's type and row size
+template <typename F>
+int dispatch(const wkv6_token_logits *p, F f) {
+    const int threads = row_threads(p);
+    auto typed = [&](auto *t) {
+        if (threads == 32) return f(std::integral_constant<int, 32>{}, t);
+        if (threads == 128) return f(std::integral_constant<int, 128>{}, t);
+        return f(std::integral_constant<int, kRowThreads>{}, t);
+    };
+    if (p->dtype == WKV6_BF16) return typed(static_cast<__nv_bfloat16 *>(nullptr));
+    if (p->dtype == WKV6_F16) return typed(static_cast<__half *>(nullptr));
+    return typed(static_cast<float *>(nullptr));
+}
 
 int rows_of(const wkv6_token_logits *p, Rows *a, const char *what, bool need_logits) {
     if (p == nullptr) return fail(WKV6_ERR_INVALID, "%s: NULL argument", what);
@@ -514,27 +715,21 @@ int rows_of(const wkv6_token_logits *p, Rows *a, const char *what, bool need_log
     a->mask = p->mask;
     a->k = (float)(1.4426950408889634 / (double)p->temperature);
     a->inv_tau = (float)(1.0 / (double)p->temperature);
+    a->low = -FLT_MAX / 4.f / fmaxf(a->k, 1.f);
     return WKV6_OK;
 }
-
-bool warp_rows(const wkv6_token_logits *p) { return (int64_t)p->V * (int64_t)dtype_size(p->dtype) <= kWarpRowBytes; }
 
 template <bool POLICY>
 int launch_rows(const wkv6_token_logits *p, const Rows &a, float *lp, float2 *stat, const Policy &q, float *coefficient, void *g,
                 cudaStream_t st) {
-    const bool warp = warp_rows(p);
-    const unsigned grid = (unsigned)(warp ? (a.rows + kWarpRows - 1) / kWarpRows : a.rows);
-#define LAUNCH(T)                                                                                                                   \
-    if (warp) token_rows_kernel<T, 32, POLICY><<<grid, 32 * kWarpRows, 0, st>>>(a, lp, stat, q, coefficient, static_cast<T *>(g)); \
-    else token_rows_kernel<T, kRowThreads, POLICY><<<grid, kRowThreads, 0, st>>>(a, lp, stat, q, coefficient, static_cast<T *>(g))
-    switch (p->dtype) {
-        case WKV6_BF16: LAUNCH(__nv_bfloat16); break;
-        case WKV6_F16: LAUNCH(__half); break;
-        default: LAUNCH(float); break;
-    }
-#undef LAUNCH
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? WKV6_OK : cuda_fail(e, "token_rows_kernel launch");
+    return dispatch(p, [&](auto size, auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        constexpr int threads = size.value;
+        const unsigned grid = (unsigned)(threads == 32 ? (a.rows + kWarpRows - 1) / kWarpRows : a.rows);
+        token_rows_kernel<T, threads, POLICY><<<grid, threads == 32 ? 32 * kWarpRows : threads, 0, st>>>(a, lp, stat, q, coefficient, static_cast<T *>(g));
+        const cudaError_t e = cudaGetLastError();
+        return e == cudaSuccess ? (int)WKV6_OK : cuda_fail(e, "token_rows_kernel launch");
+    });
 }
 
 int64_t count_parts(int64_t S, int64_t T, int reduction) {
@@ -564,24 +759,18 @@ extern "C" int wkv6_token_log_probs_backward(const wkv6_token_logits *p, const f
     if (!stat || !coefficient || !g || (unless_one && !factor)) return fail(WKV6_ERR_INVALID, "wkv6_token_log_probs_backward: NULL argument");
     if (!aligned16(g) || reinterpret_cast<uintptr_t>(stat) % 8)
         return fail(WKV6_ERR_INVALID, "wkv6_token_log_probs_backward: the gradient must be 16-byte aligned, stat 8-byte");
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool warp = warp_rows(p);
-    constexpr int threads = 256;
-    // parts of at least two vectors a thread, as many as four blocks per SM need
-    const int64_t want = (4LL * sm_count() + a.rows - 1) / a.rows, most = (int64_t)a.V * (int64_t)dtype_size(p->dtype) / (threads * 32) + 1;
-    const dim3 grid((unsigned)(warp ? (a.rows + kWarpRows - 1) / kWarpRows : a.rows), (unsigned)(warp ? 1 : want < most ? want : most));
-    const float2 *s = reinterpret_cast<const float2 *>(stat);
-#define LAUNCH(T)                                                                                                                            \
-    if (warp) token_gradient_kernel<T, 32><<<grid, 32 * kWarpRows, 0, st>>>(a, s, coefficient, per_sequence, factor, unless_one, static_cast<T *>(g)); \
-    else token_gradient_kernel<T, threads><<<grid, threads, 0, st>>>(a, s, coefficient, per_sequence, factor, unless_one, static_cast<T *>(g))
-    switch (p->dtype) {
-        case WKV6_BF16: LAUNCH(__nv_bfloat16); break;
-        case WKV6_F16: LAUNCH(__half); break;
-        default: LAUNCH(float); break;
-    }
-#undef LAUNCH
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? WKV6_OK : cuda_fail(e, "token_gradient_kernel launch");
+    return dispatch(p, [&](auto size, auto *t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        constexpr int threads = size.value;
+        // parts of at least one stage, as many as it takes to give every SM its blocks
+        const int64_t want = ((int64_t)row_blocks(threads) * sm_count() + a.rows - 1) / a.rows;
+        const int64_t most = (int64_t)p->V * (int64_t)sizeof(T) / (threads * kU * 16) + 1;
+        const dim3 grid((unsigned)(threads == 32 ? (a.rows + kWarpRows - 1) / kWarpRows : a.rows), (unsigned)(threads == 32 ? 1 : want < most ? want : most));
+        token_gradient_kernel<T, threads><<<grid, threads == 32 ? 32 * kWarpRows : threads, 0, static_cast<cudaStream_t>(stream)>>>(
+            a, reinterpret_cast<const float2 *>(stat), coefficient, per_sequence, factor, unless_one, static_cast<T *>(g));
+        const cudaError_t e = cudaGetLastError();
+        return e == cudaSuccess ? (int)WKV6_OK : cuda_fail(e, "token_gradient_kernel launch");
+    });
 }
 
 extern "C" size_t wkv6_policy_loss_workspace_bytes(int32_t S, int32_t T, int32_t reduction) {
