@@ -68,6 +68,8 @@ def parse():
                          "optimizer step of the 1.6B-shape RWKV-6 model (24 layers, d 2048, ffn 7168, vocab 65536, B8 T4096 per "
                          "GPU, bf16, AdamW, data parallel with NCCL gradient all-reduce when launched on several GPUs)")
     ap.add_argument("--no-checkpoint", action="store_true", help="train_step: keep all activations instead of recomputing blocks")
+    ap.add_argument("--optimizer", default="torch", choices=["torch", "b200", "b200-8bit"],
+                    help="train_step: the framework's fused AdamW, or this package's with fp32 or 8-bit states and stochastically rounded bf16 weights")
     ap.add_argument("--framework-loss", action="store_true",
                     help="train_step: torch's cross_entropy on an fp32 copy of the logits instead of the fused loss kernel")
     ap.add_argument("--decode-steps", type=int, default=256, help="inference: greedy decode steps after the prefill")
@@ -1074,7 +1076,11 @@ def run_train_step(a):
     net = model
     if world > 1:
         net = torch.nn.parallel.DistributedDataParallel(model, device_ids=[local], gradient_as_bucket_view=True)
-    opt = torch.optim.AdamW(model.parameters(), lr=1e-4, fused=True)
+    if a.optimizer == "torch":
+        opt = torch.optim.AdamW(model.parameters(), lr=1e-4, fused=True)
+    else:
+        from star_rwkv6_b200.optim import AdamW
+        opt = AdamW(model.parameters(), lr=1e-4, state_bits=8 if a.optimizer == "b200-8bit" else 32)
     g = torch.Generator().manual_seed(1 + rank)
     host = [torch.randint(0, V, (B, T + 1), generator=g).pin_memory() for _ in range(2)]
     ckpt = not a.no_checkpoint
@@ -1128,7 +1134,7 @@ def run_train_step(a):
             "warmup": max(3, a.warmup), "ms_per_step": ms, "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
             "dtype": "bf16", "data": "synthetic",
             "config": {"workload": f"RWKV-6 training step: {L} layers, d_model {D}, ffn {FF}, vocab {V}, B{B} T{T} per GPU, AdamW",
-                       "parameters": nparams, "block_recomputation": ckpt, "last_loss": last,
+                       "parameters": nparams, "block_recomputation": ckpt, "last_loss": last, "optimizer": a.optimizer,
                        "loss": "framework cross_entropy on fp32 logits" if a.framework_loss else "fused softmax cross-entropy + logit gradient on bf16 logits",
                        "parallelism": f"dp{world}" + (" (DDP, NCCL bucketed all-reduce overlapped with the backward)" if world > 1 else "")},
             "roofline": {"bound": "tensor", "kernel": "whole step (library GEMMs dominate)", "achieved": ach, "peak": peak,

@@ -222,10 +222,7 @@ __device__ __forceinline__ void gradient_loose(const T *z, T *out, const Cut &l,
     }
 }
 
-#ifndef TL_U
-#define TL_U 4
-#endif
-constexpr int kU = TL_U;         // vectors that a thread requests at once, while it computes on as many
+constexpr int kU = 4;         // vectors that a thread requests at once, while it computes on as many
 
 // Logits that are read once leave no line in the first-level cache; KEEP (the row will be read again): nor do the others, but with that
 // hint they also leave the second-level cache early (policy loss at 8192 x 65536: 340 MB read per 198 MB of rows, and 450 us for 392).
@@ -391,7 +388,8 @@ __device__ __forceinline__ const T *row_of(const Rows &a, int64_t row) {
 // The row's target, or -1 where the row does not count.
 __device__ __forceinline__ int target_of(const Rows &a, int64_t row) {
     const int64_t t = a.targets[row];
-    return (a.mask == nullptr || a.mask[row]) && t >= 0 && t < a.V ? (int)t : -1;
+    const uint8_t counts = a.mask != nullptr ? a.mask[row] : 1;      // on its way together with the target
+    return counts && t >= 0 && t < a.V ? (int)t : -1;
 }
 
 // What the policy loss takes beside the rows.
@@ -432,10 +430,7 @@ __device__ __forceinline__ void total_loss(const Policy &q, int64_t rows, const 
     }
 }
 
-#ifndef TL_THREADS
-#define TL_THREADS 256
-#endif
-constexpr int kRowThreads = TL_THREADS;     // of a long row
+constexpr int kRowThreads = 256;     // of a long row
 __host__ __device__ constexpr int row_blocks(int threads) { return 1024 / (threads == 32 ? 32 * kWarpRows : threads); }   // per SM
 
 // What a row's loss takes beside its log-probability, requested before the row.
@@ -510,9 +505,9 @@ token_rows_kernel(const Rows a, float *__restrict__ lp_out, float2 *__restrict__
         Part r{a.low, a.low * a.k, 0.f};
         bool wide = false;
         Batches x;
+        Terms t;
+        if constexpr (POLICY) t = terms_of(a, q, row);
         if (target >= 0) {
-            Terms t;
-            if constexpr (POLICY) t = terms_of(a, q, row);
             const float zt = Vec<T>::get1(z[target]);
             row_part<T, THREADS, POLICY>(share, a.k, r, x);
             take_loose(z, l, tid, THREADS, a.k, r);
@@ -564,13 +559,15 @@ template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, row_blocks(THREADS))
 token_gradient_kernel(const Rows a, const float2 *__restrict__ stat, const float *__restrict__ coefficient, int per_sequence,
                       const float *__restrict__ factor, int unless_one, T *__restrict__ g) {
-    const float f = factor != nullptr ? *factor : 1.f;
-    if (unless_one && f == 1.f) return;
     const int64_t row = THREADS == 32 ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= a.rows) return;
-    const int tid = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x, first = blockIdx.y * THREADS + tid, step = THREADS * gridDim.y;
+    // everything small is requested at once
+    const float f = factor != nullptr ? *factor : 1.f, per_row = coefficient[per_sequence ? (uint32_t)row / (uint32_t)a.T : row];
+    const float2 s = stat[row];
     const int target = target_of(a, row);
-    const float gc = target < 0 ? 0.f : coefficient[per_sequence ? (uint32_t)row / (uint32_t)a.T : row] * f * a.inv_tau;
+    if (unless_one && f == 1.f) return;
+    const int tid = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x, first = blockIdx.y * THREADS + tid, step = THREADS * gridDim.y;
+    const float gc = target < 0 ? 0.f : per_row * f * a.inv_tau;
     const T *z = row_of<T>(a, row);
     T *gr = g + row * a.V;
     const Cut l = cut_of(gr, a.V);
@@ -578,7 +575,6 @@ token_gradient_kernel(const Rows a, const float2 *__restrict__ stat, const float
         row_zero(gr, l, first, step);
         return;
     }
-    const float2 s = stat[row];
     if (signbit(s.y)) {
         row_gradient_direct<T, true>(z, gr, l, target, a.k, s.x, gc * s.y, gc, first, step);
     } else if ((reinterpret_cast<uintptr_t>(z) - reinterpret_cast<uintptr_t>(gr)) % 16 == 0) {

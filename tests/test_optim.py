@@ -84,9 +84,11 @@ def _check(l, i, bits, stochastic, want, random, sizes):
     for key, x in (("m", m), ("v", root)):
         scale = _flat(l[key + "s"][i])
         assert (np.abs(scale - O.block_scales(x)) <= 2.0 ** -21 * scale).all()
-        q = np.divide(x, np.repeat(O.block_scales(x), 256)[:len(x)])
+        unit = np.repeat(O.block_scales(x), 256)[:len(x)]
+        unit = np.where(unit > 0, unit, 1.0)                 # a block of zeros
+        q = x / unit
         form = O.e4m3_nearest if key == "m" else (lambda y: O.e4m3_stochastic(np.maximum(y, 0.0), random))
-        size = np.divide(terms if key == "m" else root, np.repeat(O.block_scales(x), 256)[:len(x)])
+        size = (terms if key == "m" else root) / unit
         _one_of(_flat(l[key][i]), form, q, 2.0 ** -20 * np.maximum(np.abs(q), size))
 
 
