@@ -269,7 +269,9 @@ WKV6_API int wkv6_token_log_probs_backward(const wkv6_token_logits *p, const flo
  * workspace: wkv6_policy_loss_workspace_bytes(S, T, reduction) bytes.  Sums run in a fixed order. */
 enum { WKV6_MEAN = 0, WKV6_SEQUENCE_MEAN = 1, WKV6_SUM = 2 };
 typedef struct {
-    const float *advantages, *old_log_probs;   /* [S, T] */
+    const float *advantages;                   /* of token (s, t) at s * advantage_seq_stride + t * advantage_row_stride (elements; 0: */
+    int64_t advantage_seq_stride, advantage_row_stride;   /* broadcast, as where a whole answer has one) */
+    const float *old_log_probs;                /* [S, T] */
     const float *ref_log_probs;                /* [S, T]; may be NULL when kl_coef is 0 */
     double clip_low, clip_high, kl_coef, scale;
     int32_t reduction;

@@ -55,7 +55,7 @@ class TokenLogits(ctypes.Structure):
 
 class Policy(ctypes.Structure):
     _fields_ = [
-        ("advantages", ctypes.c_void_p), ("old_log_probs", ctypes.c_void_p), ("ref_log_probs", ctypes.c_void_p),
+        ("advantages", ctypes.c_void_p), ("advantage_seq_stride", ctypes.c_int64), ("advantage_row_stride", ctypes.c_int64), ("old_log_probs", ctypes.c_void_p), ("ref_log_probs", ctypes.c_void_p),
         ("clip_low", ctypes.c_double), ("clip_high", ctypes.c_double), ("kl_coef", ctypes.c_double), ("scale", ctypes.c_double),
         ("reduction", ctypes.c_int32),
     ]

@@ -395,6 +395,7 @@ __device__ __forceinline__ int target_of(const Rows &a, int64_t row) {
 // What the policy loss takes beside the rows.
 struct Policy {
     const float *advantages, *old_lp, *ref_lp;
+    int64_t adv_seq, adv_row;      // strides of the advantages
     float low, high, kl, scale;
     int reduction;
     const int *counts;       // live rows of each part
@@ -440,13 +441,14 @@ struct Terms {
 };
 __device__ __forceinline__ Terms terms_of(const Rows &a, const Policy &q, int64_t row) {
     Terms t;
-    t.adv = q.advantages[row];
+    const uint32_t s = (uint32_t)row / (uint32_t)a.T;
+    t.adv = q.advantages[s * q.adv_seq + ((uint32_t)row - s * (uint32_t)a.T) * q.adv_row];
     t.old = q.old_lp[row];
     if (q.ref_lp != nullptr) t.ref = q.ref_lp[row];
     if (q.reduction == WKV6_MEAN)
         for (int i = threadIdx.x & 31; i < q.parts; i += 32) t.n += q.counts[i];
     else if (q.reduction == WKV6_SEQUENCE_MEAN)
-        t.n = q.counts[(uint32_t)row / (uint32_t)a.T];
+        t.n = q.counts[s];
     return t;
 }
 
@@ -483,7 +485,11 @@ __device__ __forceinline__ float finish_row(const Rows &a, const T *z, float zt,
         gather<THREADS, 1>(r.c, r.sum, a.k);
         return (zt - r.c) * a.inv_tau - logf(r.sum);
     }
-    return (fmaf(zt, a.k, -r.c) - log2f(r.sum)) * 0.69314718055994531f;
+    // The logarithm's whole part is taken off first, which is exact or nearly so: only a part in [0, 1) is off by its rounding.  (r.sum is
+    // at least about 1; the last term is 0, or NaN where the sum is.)
+    const uint32_t bits = __float_as_uint(r.sum);
+    const float whole = (float)((int)(bits >> 23) - 127), part = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
+    return ((fmaf(zt, a.k, -r.c) - whole) - log2f(part)) * 0.69314718055994531f + (r.sum - r.sum);
 }
 
 // THREADS = 32: a warp per row, several to a block (rows of a few KB, where a block's reduction would cost more than its row);
@@ -794,7 +800,10 @@ extern "C" int wkv6_policy_loss(const wkv6_token_logits *p, const wkv6_policy *c
         return fail(WKV6_ERR_WORKSPACE, "wkv6_policy_loss: workspace of %zu bytes, %zu are needed", workspace_bytes,
                     wkv6_policy_loss_workspace_bytes(p->S, p->T, c->reduction));
     Policy q{};
+    if (c->advantage_seq_stride < 0 || c->advantage_row_stride < 0) return fail(WKV6_ERR_INVALID, "wkv6_policy_loss: negative strides");
     q.advantages = c->advantages;
+    q.adv_seq = c->advantage_seq_stride;
+    q.adv_row = c->advantage_row_stride;
     q.old_lp = c->old_log_probs;
     q.ref_lp = c->kl_coef != 0.0 ? c->ref_log_probs : nullptr;
     if (c->kl_coef != 0.0 && c->ref_log_probs == nullptr) return fail(WKV6_ERR_INVALID, "wkv6_policy_loss: a KL term needs ref_log_probs");

@@ -173,6 +173,9 @@ PolicyResult policy(const Rows &r, const Tensor &targets, const PolicyCall &c, b
     Tensor ws = bytes(nbytes, r.z);
     wkv6_policy q{};
     q.advantages = ptr(c.advantages);
+    const int64_t d = c.advantages.dim();
+    q.advantage_row_stride = d > 0 ? c.advantages.stride(d - 1) : 0;
+    q.advantage_seq_stride = d == 2 ? c.advantages.stride(0) : r.T * q.advantage_row_stride;
     q.old_log_probs = ptr(c.old_lp);
     q.ref_log_probs = ptr(c.ref_lp);
     q.clip_low = c.low;
@@ -290,8 +293,8 @@ bool tensor_arg(PyObject *o, Tensor &t, bool optional) {
     return true;
 }
 
-// A constant of the loss: fp32, dense, of these sizes
-bool constant_arg(PyObject *o, Tensor &t, at::IntArrayRef sizes, const Tensor &logits, bool optional) {
+// A constant of the loss: fp32, of these sizes; dense, or (strided) with strides for the sequence and the token
+bool constant_arg(PyObject *o, Tensor &t, at::IntArrayRef sizes, const Tensor &logits, bool optional, bool strided = false) {
     if (!tensor_arg(o, t, optional)) return false;
     if (!t.defined()) return true;
     if (!at::isFloatingType(t.scalar_type()) || t.sizes() != sizes || t.device() != logits.device()) return false;
@@ -299,7 +302,8 @@ bool constant_arg(PyObject *o, Tensor &t, at::IntArrayRef sizes, const Tensor &l
         if (at::GradMode::is_enabled()) return false;
         t = t.detach();
     }
-    if (t.scalar_type() != at::kFloat || !t.is_contiguous()) t = t.to(at::kFloat).contiguous();
+    if (t.scalar_type() != at::kFloat) t = t.to(at::kFloat);
+    if (!t.is_contiguous() && !(strided && t.dim() <= 2)) t = t.contiguous();
     return true;
 }
 
@@ -359,7 +363,7 @@ PyObject *py_policy_loss(PyObject *, PyObject *const *args, Py_ssize_t n) {
         return none();
     given.temperature = x[0];
     if (!describe(logits, given, r)) return none();
-    if (!constant_arg(args[3], c.advantages, given.targets.sizes(), logits, false) || !constant_arg(args[4], c.old_lp, given.targets.sizes(), logits, false) ||
+    if (!constant_arg(args[3], c.advantages, given.targets.sizes(), logits, false, true) || !constant_arg(args[4], c.old_lp, given.targets.sizes(), logits, false) ||
         !constant_arg(args[5], c.ref_lp, given.targets.sizes(), logits, true))
         return none();
     c.low = x[1];

@@ -13,6 +13,7 @@ The gradient is written over the logits inside the forward call: the logits tens
 sampled or compared answers.  They leave the logits alone, take bf16, fp16 and fp32 logits of any vocabulary, and compute in fp32.
 Tokens that ``mask`` leaves out, and those whose target lies outside [0, V), do not count: their logits are not read, their
 log-probability is 0 and their gradient zeros.  A row that counts and holds a NaN or +inf, or nothing but -inf, gives NaN.
+Forward and backward can be captured into a CUDA graph; as with every backward pass, no eager graph of the same leaves may be alive then.
 """
 from __future__ import annotations
 
@@ -90,8 +91,8 @@ def _check_targets(logits, targets, mask, temperature):
         raise ValueError("more than 2^31 - 1 tokens, or entries of the vocabulary")
 
 
-def _per_token(t, name, targets):
-    """A constant that goes with every token, as a dense fp32 tensor."""
+def _per_token(t, name, targets, strided=False):
+    """A constant that goes with every token, in fp32; dense, or (strided) with strides for the sequence and the token."""
     _check_cuda(t)
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} is a constant of the loss: pass it without requires_grad (detach it)")
@@ -101,7 +102,8 @@ def _per_token(t, name, targets):
         raise ValueError(f"{name} {tuple(t.shape)} does not fit targets {tuple(targets.shape)}")
     if t.device != targets.device:
         raise ValueError(f"{name} must be on the logits' device")
-    return t.detach().to(torch.float32).contiguous()
+    t = t.detach().to(torch.float32)
+    return t if strided and t.dim() > 0 and (t.dim() <= 2 or t.is_contiguous()) else t.contiguous()
 
 
 def _sequences(t):
@@ -180,6 +182,8 @@ def _policy(logits, targets, mask, temperature, consts, numbers, reduction, want
     dev = logits.device
     c = Policy()
     c.advantages, c.old_log_probs, c.ref_log_probs = (0 if t is None else t.data_ptr() for t in consts)
+    c.advantage_row_stride = consts[0].stride(-1) if consts[0].dim() > 0 else 0
+    c.advantage_seq_stride = p.T * c.advantage_row_stride if consts[0].dim() != 2 else consts[0].stride(0)
     c.clip_low, c.clip_high, c.kl_coef, c.scale = numbers
     c.reduction = reduction
     loss = torch.empty((), dtype=torch.float32, device=dev)
@@ -245,7 +249,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
     if out is not None:
         return out
     _check_targets(logits, targets, mask, temperature)
-    consts = (_per_token(advantages, "advantages", targets), _per_token(old_log_probs, "old_log_probs", targets),
+    consts = (_per_token(advantages, "advantages", targets, strided=True), _per_token(old_log_probs, "old_log_probs", targets),
               _per_token(ref_log_probs, "ref_log_probs", targets) if ref_log_probs is not None else None)
     args = (logits, targets, mask, temperature, consts, (clip_low, clip_high, kl_coef, scale), _REDUCTIONS[reduction])
     if torch.is_grad_enabled() and logits.requires_grad:

@@ -109,6 +109,10 @@ def test_policy_loss(S, T, V, dtype, kl, tau, reduction):
     with torch.no_grad():
         plain = policy_loss(zc, *args, **kw)
     assert torch.equal(plain[0], got) and torch.equal(plain[1], got_lp)
+    wide = torch.zeros(T, 2 * S, device="cuda").t()[::2]     # advantages with strides of their own, of another type
+    wide.copy_(args[1])
+    for a in (args[1].contiguous(), wide, args[1].double()):
+        assert torch.equal(policy_loss(zc, args[0], a, args[2], **kw)[0], got)
 
 
 @pytest.mark.gpu
@@ -423,4 +427,4 @@ def test_refusals_of_the_library():
     assert lib.wkv6_preference_loss(rows(S=3), a, q, a, a, a, a, 100, None) == -1
     assert lib.wkv6_preference_loss(rows(), a, q, a, a, a, a, 23, None) == -3
     assert lib.wkv6_preference_loss(rows(), None, q, a, a, a, a, 24, None) == -1
-    assert ctypes.sizeof(L.TokenLogits) == 64 and ctypes.sizeof(L.Policy) == 64 and ctypes.sizeof(L.Preference) == 48
+    assert ctypes.sizeof(L.TokenLogits) == 64 and ctypes.sizeof(L.Policy) == 80 and ctypes.sizeof(L.Preference) == 48
