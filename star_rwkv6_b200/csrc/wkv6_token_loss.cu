@@ -148,7 +148,8 @@ __device__ __forceinline__ void take(const uint4 (&q)[U], float k, Part &r) {
 #pragma unroll
     for (int u = 0; u < U; ++u) m = fmaxf(m, Vec<T>::max(q[u]));
     const float c = m * k;
-    float sum0 = r.sum * ex2(r.c - c), sum1 = 0.f;
+    const float scale = ex2(r.c - c);
+    float sum0 = 0.f, sum1 = 0.f;      // not the whole sum: next to a large term in it, each of hundreds of small ones would be rounded
     r.mx = m;
     r.c = c;
 #pragma unroll
@@ -161,7 +162,7 @@ __device__ __forceinline__ void take(const uint4 (&q)[U], float k, Part &r) {
             sum1 += ex2(fmaf(f[e].y, k, -c));
         }
     }
-    r.sum = sum0 + sum1;
+    r.sum = fmaf(r.sum, scale, sum0 + sum1);
 }
 
 // g (1[j = a] - p_j) of a vector of logits: neg = -g / sum, `at` = a's place in the vector.  (Products and sums are kept apart, so that all
