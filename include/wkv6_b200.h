@@ -246,7 +246,7 @@ WKV6_API int wkv6_scale_bf16(int64_t n, void *g, const float *scale, void *strea
 typedef struct {
     int32_t S, T, V;
     int32_t dtype;                       /* logits and their gradient: WKV6_BF16, WKV6_F16, WKV6_F32; aligned to one element */
-    float temperature;                   /* > 0 */
+    float temperature;                   /* at least 1e-30 */
     int64_t seq_stride, row_stride;
     const void *logits;
     const int64_t *targets;
@@ -304,7 +304,7 @@ WKV6_API int wkv6_preference_loss(const wkv6_token_logits *p, const float *log_p
  * step).  stochastic: bf16 parameters are rounded the same way, from 16 random bits each; otherwise to nearest.  The random bits are
  * a function of seed, t, the tensor's `index` and the value's place in it.
  * A gradient that is infinite or NaN makes its value NaN (8 bits: its block's moments too).
- * t is `step`, or *step_device where that is not NULL; lr is `lr`, or *lr_device.  Tensors must not overlap; n == 0 is allowed.
+ * t is `step`, or *step_device where that is not NULL (at least 1); lr is `lr`, or *lr_device.  Tensors must not overlap; n == 0 is allowed.
  * No counterpart in the reference (its trainer files are empty).
  */
 typedef struct {

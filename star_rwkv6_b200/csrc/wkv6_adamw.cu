@@ -1,10 +1,13 @@
 // AdamW over many tensors at once (include/wkv6_b200.h gives the formulas), states in fp32 or in blocks of 256 e4m3 codes with a scale.
 //
-// Bound by HBM: a bf16 value with fp32 states moves 22 bytes, with 8-bit states 10.06, for about twenty operations.  The tensors of a
-// model differ in size by four orders of magnitude, so they are cut into chunks of 2048 values and the blocks of one launch walk all
-// chunks; a chunk's tensor is found by bisection in a table that travels in the launch's arguments (no copy to the device, nothing to
+// A bf16 value with fp32 states moves 22 bytes, with 8-bit states 10.06.  The first is bound by HBM: 368 M values (two layers, embedding
+// and head of the 1.6B shape) in 1328 us, 96 % of the copy bandwidth.  The second is bound by instructions: 896 us, 65 % of it, at 64.6
+// instructions per value (at the copy bandwidth there is time for 55): random bits, two square roots' and two conversions' worth of
+// work per value, and moments that keep the bits of elementary operations.
+// The tensors of a model differ in size by four orders of magnitude, so they are cut into chunks and the blocks of one launch share all
+// chunks; a chunk's tensor is found in a table that travels in the launch's arguments (no copy to the device, nothing to
 // keep alive, and a captured launch holds its own).  A thread has eight neighbouring values, a warp the 256 of a block of codes, whose
-// largest value is one warp reduction.
+// largest value is one warp reduction.  The next chunk's values are requested before this one's are computed.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -18,14 +21,10 @@ namespace wkv6 {
 
 namespace {
 
-#ifndef ADAMW_BLOCKS
-#define ADAMW_BLOCKS 2
-#endif
-#ifndef ADAMW_G
-#define ADAMW_G 2
-#endif
-constexpr int kThreads = 256, kPerThread = 8, kGroupValues = kThreads * kPerThread, kBlock = 256, kBlocksPerSm = ADAMW_BLOCKS;
-__host__ __device__ constexpr int groups(int bits) { return bits == 8 ? ADAMW_G : 1; }     // of eight values per thread and chunk
+// Two blocks per SM: with the next chunk's values in registers a thread needs 112 to 118 of them.  Measured for 368 M bf16 values: fp32
+// states 1328 us (three blocks 1519, four 1602); 8 bits 896 us with 16 values per thread and chunk (eight: 1017; not requested ahead: 983).
+constexpr int kThreads = 256, kPerThread = 8, kGroupValues = kThreads * kPerThread, kBlock = 256, kBlocksPerSm = 2;
+__host__ __device__ constexpr int groups(int bits) { return bits == 8 ? 2 : 1; }     // of eight values per thread and chunk
 
 struct Entry {
     void *p;
@@ -231,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) adamw_kernel(const __g
     int64_t t = a.step;
     if (a.step_device != nullptr || a.lr_device != nullptr) {
         const double lr = a.lr_device != nullptr ? (double)*a.lr_device : a.lr;
-        if (a.step_device != nullptr) t = *a.step_device;
+        if (a.step_device != nullptr) t = max((long long)*a.step_device, 1ll);
         if (threadIdx.x == 0) {
             shared[0] = (float)(lr / (1.0 - power(a.beta1, t)));
             shared[1] = (float)(1.0 / sqrt(1.0 - power(a.beta2, t)));

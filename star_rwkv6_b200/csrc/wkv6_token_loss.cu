@@ -703,7 +703,7 @@ int rows_of(const wkv6_token_logits *p, Rows *a, const char *what, bool need_log
     if (p == nullptr) return fail(WKV6_ERR_INVALID, "%s: NULL argument", what);
     if (p->S < 0 || p->T < 0 || p->V < 1) return fail(WKV6_ERR_INVALID, "%s: S=%d T=%d V=%d", what, p->S, p->T, p->V);
     if (p->dtype != WKV6_BF16 && p->dtype != WKV6_F16 && p->dtype != WKV6_F32) return fail(WKV6_ERR_INVALID, "%s: unknown dtype code", what);
-    if (!(p->temperature > 0.f) || std::isinf(p->temperature)) return fail(WKV6_ERR_INVALID, "%s: temperature must be positive and finite", what);
+    if (!(p->temperature >= 1e-30f) || std::isinf(p->temperature)) return fail(WKV6_ERR_INVALID, "%s: temperature must be at least 1e-30 and finite", what);
     a->rows = (int64_t)p->S * p->T;
     if (a->rows > 2147483647LL) return fail(WKV6_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 tokens", what);
     a->T = p->T;

@@ -56,7 +56,7 @@ bool describe(const Tensor &logits, const Given &given, Rows &r) {
     const int64_t d = logits.dim();
     if (d < 1 || targets.dim() != d - 1 || dtype_code(logits.scalar_type()) < 0 || targets.scalar_type() != at::kLong) return false;
     const int64_t V = logits.size(d - 1), rows = targets.numel();
-    if (V < 1 || V >= (1LL << 31) || rows < 1 || rows >= (1LL << 31) || !(temperature > 0.0) || std::isinf(temperature)) return false;
+    if (V < 1 || V >= (1LL << 31) || rows < 1 || rows >= (1LL << 31)) return false;
     if (!std::equal(targets.sizes().begin(), targets.sizes().end(), logits.sizes().begin()) || targets.device() != logits.device()) return false;
     if (mask.defined() && (mask.scalar_type() != at::kBool || mask.sizes() != targets.sizes() || mask.device() != logits.device())) return false;
     if (V > 1 && logits.stride(d - 1) != 1) return false;
@@ -73,7 +73,7 @@ bool describe(const Tensor &logits, const Given &given, Rows &r) {
     r.p.V = (int32_t)V;
     r.p.dtype = dtype_code(logits.scalar_type());
     r.p.temperature = (float)temperature;
-    if (!(r.p.temperature > 0.f) || std::isinf(r.p.temperature)) return false;
+    if (!(r.p.temperature >= 1e-30f) || std::isinf(r.p.temperature)) return false;
     r.p.row_stride = row;
     r.p.seq_stride = seq;
     r.p.logits = logits.const_data_ptr();
@@ -173,9 +173,9 @@ PolicyResult policy(const Rows &r, const Tensor &targets, const PolicyCall &c, b
     Tensor ws = bytes(nbytes, r.z);
     wkv6_policy q{};
     q.advantages = ptr(c.advantages);
-    const int64_t d = c.advantages.dim();
-    q.advantage_row_stride = d > 0 ? c.advantages.stride(d - 1) : 0;
-    q.advantage_seq_stride = d == 2 ? c.advantages.stride(0) : r.T * q.advantage_row_stride;
+    const int64_t d = c.advantages.dim();      // more than two: dense
+    q.advantage_row_stride = d == 1 || d == 2 ? c.advantages.stride(d - 1) : 1;
+    q.advantage_seq_stride = d == 2 ? c.advantages.stride(0) : r.T;
     q.old_log_probs = ptr(c.old_lp);
     q.ref_log_probs = ptr(c.ref_lp);
     q.clip_low = c.low;

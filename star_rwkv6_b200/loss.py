@@ -85,8 +85,8 @@ def _check_targets(logits, targets, mask, temperature):
     for t in (targets, mask):
         if t is not None and t.device != logits.device:
             raise ValueError("logits, targets and mask must be on one device")
-    if not (temperature > 0.0 and math.isfinite(temperature)):
-        raise ValueError("temperature must be positive and finite")
+    if not (temperature >= 1e-30 and math.isfinite(temperature)):
+        raise ValueError("temperature must be at least 1e-30 and finite")
     if targets.numel() >= 2 ** 31 or logits.shape[-1] >= 2 ** 31:
         raise ValueError("more than 2^31 - 1 tokens, or entries of the vocabulary")
 
@@ -182,8 +182,9 @@ def _policy(logits, targets, mask, temperature, consts, numbers, reduction, want
     dev = logits.device
     c = Policy()
     c.advantages, c.old_log_probs, c.ref_log_probs = (0 if t is None else t.data_ptr() for t in consts)
-    c.advantage_row_stride = consts[0].stride(-1) if consts[0].dim() > 0 else 0
-    c.advantage_seq_stride = p.T * c.advantage_row_stride if consts[0].dim() != 2 else consts[0].stride(0)
+    d = consts[0].dim()                       # more than two: dense
+    c.advantage_row_stride = consts[0].stride(-1) if d in (1, 2) else 1
+    c.advantage_seq_stride = consts[0].stride(0) if d == 2 else p.T
     c.clip_low, c.clip_high, c.kl_coef, c.scale = numbers
     c.reduction = reduction
     loss = torch.empty((), dtype=torch.float32, device=dev)

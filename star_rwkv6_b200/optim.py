@@ -162,6 +162,8 @@ class AdamW(torch.optim.Optimizer):
         if not s:
             if group["capturable"] and group["step"] is not None:
                 raise RuntimeError("a capturable group's parameters must have gradients from its first step on")
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("take a first step before the capture: new states would be zeroed at every replay")
             if group["state_bits"] == 32:
                 s["exp_avg"], s["exp_avg_sq"] = (torch.zeros(p.shape, dtype=torch.float32, device=p.device) for _ in range(2))
             else:
@@ -188,13 +190,13 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError("AdamW does not take sparse gradients")
                 s = self._state_of(p, group)
                 batches.setdefault((p.device, s["step"]), []).append((p, s))
-            for (device, at), batch in batches.items():
-                if group["capturable"]:
-                    if group["step"] is None:
-                        group["step"] = torch.zeros((), dtype=torch.int64, device=device)
-                    elif group["step"].device != device:
-                        raise RuntimeError("a capturable group's parameters must be on one device")
-                    group["step"].add_(1)
+            if group["capturable"] and batches:
+                if len(batches) > 1:
+                    raise RuntimeError("a capturable group's parameters must be on one device")
+                if group["step"] is None:
+                    group["step"] = torch.zeros((), dtype=torch.int64, device=next(iter(batches))[0])
+                group["step"].add_(1)
+            for (_, at), batch in batches.items():
                 ps, ss = [p for p, _ in batch], [s for _, s in batch]
                 scales = ([s[k + "_scale"] for s in ss] for k in ("exp_avg", "exp_avg_sq")) if group["state_bits"] == 8 else (None, None)
                 m_scales, v_scales = scales

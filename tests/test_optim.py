@@ -329,6 +329,11 @@ def test_optimizer_captured():
     late.grad = torch.ones(3, device="cuda")
     with pytest.raises(RuntimeError, match="first step"):
         opt.step()
+    fresh = AdamW([late], capturable=True)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            fresh.step()
+    assert not late.any()
 
 
 @pytest.mark.gpu

@@ -338,6 +338,74 @@ def test_captured_and_on_other_streams():
 
 
 @pytest.mark.gpu
+def test_two_calls_at_once():
+    """Calls on two streams with nothing between them: each has its own workspace."""
+    from star_rwkv6_b200.loss import policy_loss, preference_loss
+    sets, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for k in range(2):
+        z, targets, mask, g = _inputs(6, 150, 2000 + 3000 * k, torch.bfloat16, seed=20 + k)
+        adv, old = torch.randn(6, 150, generator=g), torch.full((6, 150), -6.0)
+        sets.append([t.cuda() for t in (z, targets, mask, adv, old)])
+
+    def both(z, targets, mask, adv, old):
+        z = z.detach().requires_grad_(True)
+        a, lp = policy_loss(z, targets, adv, old, mask=mask)
+        b, seq = preference_loss(z, targets, None, mask)
+        return a.detach(), lp, torch.autograd.grad(a, z)[0], b.detach(), seq, torch.autograd.grad(b, z)[0]
+
+    want = [both(*s) for s in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for s, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                got.append(both(*s))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert all(torch.equal(x, y) for x, y in zip(out, want[i % 2]))
+
+
+def _outputs_of_one_run():
+    """What the native and the Python call path are compared on."""
+    from star_rwkv6_b200.loss import policy_loss, preference_loss, token_log_probs
+    from star_rwkv6_b200.optim import AdamW
+    out = []
+    for V, dtype in ((50, torch.float32), (1001, torch.bfloat16), (9000, torch.float16)):
+        z, targets, mask, g = _inputs(4, 6, V, dtype, seed=30)
+        z, targets, mask = z.cuda().requires_grad_(True), targets.cuda(), mask.cuda()
+        adv, old = torch.randn(4, 1, generator=g).cuda().expand(4, 6), torch.full((4, 6), -5.0, device="cuda")
+        lp = token_log_probs(z, targets, mask, temperature=0.9)
+        a, alp = policy_loss(z, targets, adv, old, ref_log_probs=old + 0.5, mask=mask, kl_coef=0.1, reduction="sequence_mean")
+        b, seq = preference_loss(z, targets, None, mask, average=True, margin=0.1)
+        out += [lp, alp, seq, a, b] + [torch.autograd.grad(x, z)[0] for x in (lp.sum(), a, b * 2)]
+    for bits in (32, 8):
+        torch.manual_seed(0)
+        ps = [torch.nn.Parameter(torch.randn(n, device="cuda").to(dt)) for n, dt in ((700, torch.bfloat16), (33, torch.float32), (4096, torch.bfloat16))]
+        opt = AdamW(ps, state_bits=bits, seed=3)
+        for _ in range(3):
+            for p in ps:
+                p.grad = torch.randn_like(p)
+            opt.step()
+        out += ps + [t.float() for s in opt.state.values() for t in s.values() if torch.is_tensor(t)]
+    return [t.detach().cpu() for t in out]
+
+
+@pytest.mark.gpu
+def test_both_call_paths_give_the_same_bits(tmp_path):
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = ("import sys, warnings; warnings.simplefilter('ignore'); sys.modules['star_rwkv6_b200._native'] = None\n"
+            f"sys.path[:0] = [{os.path.dirname(here)!r}, {here!r}]\nimport torch, test_token_losses as t\n"
+            f"torch.save(t._outputs_of_one_run(), {str(tmp_path / 'out.pt')!r})")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    python, native = torch.load(tmp_path / "out.pt"), _outputs_of_one_run()
+    assert len(python) == len(native) and all(torch.equal(a, b) for a, b in zip(python, native))
+
+
+@pytest.mark.gpu
 def test_derivatives_of_the_gradients_are_refused():
     from star_rwkv6_b200.loss import policy_loss, preference_loss, token_log_probs
     z = torch.randn(2, 3, 50, device="cuda", requires_grad=True)
@@ -377,7 +445,7 @@ def test_refusals():
     bad = [(TypeError, lambda: token_log_probs(z.double(), t)), (TypeError, lambda: token_log_probs(z, t.int())),
            (ValueError, lambda: token_log_probs(z, t[:, :2])), (ValueError, lambda: token_log_probs(z[..., :0], t)),
            (TypeError, lambda: token_log_probs(z, t, m.int())), (ValueError, lambda: token_log_probs(z, t, m[:1])),
-           (ValueError, lambda: token_log_probs(z, t, temperature=0.0)), (ValueError, lambda: token_log_probs(z, t, temperature=float("nan"))),
+           (ValueError, lambda: token_log_probs(z, t, temperature=0.0)), (ValueError, lambda: token_log_probs(z, t, temperature=1e-40)), (ValueError, lambda: token_log_probs(z, t, temperature=float("nan"))),
            (RuntimeError, lambda: token_log_probs(z, t.cpu())), (RuntimeError, lambda: policy_loss(z, t, x.cpu(), x)),
            (ValueError, lambda: policy_loss(z, t, x[:, :1], x)), (TypeError, lambda: policy_loss(z, t, t, x)),
            (ValueError, lambda: policy_loss(z, t, x.clone().requires_grad_(True), x)), (ValueError, lambda: policy_loss(z, t, x, x, kl_coef=0.1)),
@@ -404,7 +472,7 @@ def test_refusals_of_the_library():
             setattr(p, k, v)
         return p
 
-    for kw in (dict(S=-1), dict(V=0), dict(dtype=9), dict(temperature=0.0), dict(temperature=float("inf")), dict(logits=0), dict(targets=0),
+    for kw in (dict(S=-1), dict(V=0), dict(dtype=9), dict(temperature=0.0), dict(temperature=1e-40), dict(temperature=float("inf")), dict(logits=0), dict(targets=0),
                dict(row_stride=-8), dict(logits=a + 1)):
         assert lib.wkv6_token_log_probs(rows(**kw), a, None, None) == -1, kw
     assert lib.wkv6_token_log_probs(rows(S=70000, T=70000), a, None, None) == -2
