@@ -3,9 +3,15 @@
 //   c = k max z,   s = sum_j 2^(k z_j - c),   lp = (k z_a - c - log2 s) ln 2,   p_j = 2^(k z_j - c) / s
 //   d lp / d z_j = (1[j = a] - p_j) / tau
 // Everything is bound by the bytes of the logits (65536 of them per token), and next by instructions: at the copy bandwidth a bf16
-// logit has to be done with in 11.  A row's maximum and sum are taken in one pass (the sum is rescaled when the maximum grows), and
-// where the gradient needs nothing but the row itself (policy loss) the row is gone through again right behind that, from its end to its
-// start: the end is still in shared memory, the rest in the L2 cache.
+// logit has to be done with in 11 (it takes 6.4 forward, 15 with the gradient behind it, for which there is twice the time).  A row's
+// maximum and sum are taken in one pass (the sum is rescaled when the maximum grows), and where the gradient needs nothing but the row
+// itself (policy loss) the row is gone through again right behind that, from its end to its start: the end is still in registers, the
+// rest in the L2 cache.  A block of 256 threads has a row, four of them are on an SM: with 512 threads all warps of an SM compute or wait
+// at once (rows of 65536 bf16: 80 us instead of 71 for 2968 of them), with 128 the rows under way do not fit the L2 cache (policy loss 415
+// us instead of 375), and rows that blocks claim and request ahead through shared memory took 92 us: more instructions, nothing gained.
+// Measured, 6000 rows of 65536 bf16, all of them counting: log-probabilities 121 us = 6.48 TB/s (99 % of the copy bandwidth), their
+// gradient 249 us = 6.31 TB/s, the policy loss with its gradient 301 us = 5.23 TB/s: its second pass comes from the L2 cache, which
+// loses about a fifth of the rows under way.
 // Rows that the mask leaves out, or whose target is no token, are not read: their log-probability and gradient are zero
 // whatever the logits hold.
 // k z - c is one multiply-add: c is rounded, but it is the same c everywhere in a row, so that it cancels.  Logits near the end of the
@@ -140,20 +146,21 @@ struct Part {
     float mx, c, sum;
 };
 
-// Takes U vectors into a part.
+// Takes U vectors into a part, or the first `have` of them.
 template <typename T, int U>
-__device__ __forceinline__ void take(const uint4 (&q)[U], float k, Part &r) {
+__device__ __forceinline__ void take(const uint4 (&q)[U], float k, Part &r, int have = U) {
     constexpr int N = Vec<T>::N;
     float m = r.mx;
 #pragma unroll
     for (int u = 0; u < U; ++u) m = fmaxf(m, Vec<T>::max(q[u]));
-    const float c = m * k;
+    const float c = __fmul_rn(m, k);       // not to be contracted with a sum: c stands for itself, rounded, everywhere
     const float scale = ex2(r.c - c);
     float sum0 = 0.f, sum1 = 0.f;      // not the whole sum: next to a large term in it, each of hundreds of small ones would be rounded
     r.mx = m;
     r.c = c;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+        if (u >= have) break;
         float2 f[N / 2];
         Vec<T>::get(q[u], f);
 #pragma unroll
@@ -206,7 +213,7 @@ __device__ __forceinline__ Cut cut_of(const T *p, int V) {
 template <typename T>
 __device__ __forceinline__ void take_loose(const T *z, const Cut &l, int first, int step, float k, Part &r) {
     for (int i = first; i < l.loose; i += step) {
-        const float x = Vec<T>::get1(z[l.at(i)]), m = fmaxf(r.mx, x), c = m * k;
+        const float x = Vec<T>::get1(z[l.at(i)]), m = fmaxf(r.mx, x), c = __fmul_rn(m, k);
         r.sum = r.sum * ex2(r.c - c) + ex2(fmaf(x, k, -c));
         r.mx = m;
         r.c = c;
@@ -242,7 +249,7 @@ struct Share {
     int count;
     __device__ __forceinline__ Share(const uint4 *vectors, int n, int tid) : v(vectors + tid), count((n - tid + THREADS - 1) / THREADS) {}
     __device__ __forceinline__ int batches() const { return (count + kU - 1) / kU; }
-    // Vectors that do not exist come as -inf, which adds nothing.
+    // Vectors that do not exist come as -inf: no maximum.
     template <bool KEEP>
     __device__ __forceinline__ void load(int b, uint4 (&q)[kU]) const {
         const uint4 *p = v + (int64_t)b * (kU * THREADS);
@@ -269,12 +276,17 @@ __device__ __forceinline__ void row_part(const Share<T, THREADS> &w, float k, Pa
     int b = n & 1;
     if (b) w.template load<KEEP>(0, x.odd);
     if (n > b) w.template load<KEEP>(b, x.even);
-    if (b) take<T, kU>(x.odd, k, r);
-    for (; b < n; b += 2) {
+    if (b) take<T, kU>(x.odd, k, r, w.count);          // where it is the only one, not all of it need be there
+    for (; b + 2 < n; b += 2) {
         w.template load<KEEP>(b + 1, x.odd);
         take<T, kU>(x.even, k, r);
-        if (b + 2 < n) w.template load<KEEP>(b + 2, x.even);
+        w.template load<KEEP>(b + 2, x.even);
         take<T, kU>(x.odd, k, r);
+    }
+    if (b < n) {
+        w.template load<KEEP>(b + 1, x.odd);
+        take<T, kU>(x.even, k, r);
+        take<T, kU>(x.odd, k, r, w.count - (n - 1) * kU);
     }
 }
 
@@ -479,7 +491,7 @@ __device__ __forceinline__ float2 loss_of(const Rows &a, const Policy &q, Terms 
 template <typename T, int THREADS>
 __device__ __forceinline__ float finish_row(const Rows &a, const T *z, float zt, int tid, Part &r, bool &wide) {
     gather<THREADS, 0>(r.c, r.sum, 1.f);
-    const float end = -a.low * a.k;      // the same in all threads; a NaN in the sum stays what it is
+    const float end = -__fmul_rn(a.low, a.k);      // the same in all threads; a NaN in the sum stays what it is
     wide = !(r.c > -end && r.c < end);
     if (wide) {
         row_part_wide(z, a.V, tid, THREADS, a.k, r.c, r.sum);
@@ -509,7 +521,7 @@ token_rows_kernel(const Rows a, float *__restrict__ lp_out, float2 *__restrict__
         const Share<T, THREADS> share(reinterpret_cast<const uint4 *>(z + l.head), l.vecs, tid);
         float lp = 0.f, inv_sum = 0.f;
         float2 loss = make_float2(0.f, 0.f);
-        Part r{a.low, a.low * a.k, 0.f};
+        Part r{a.low, __fmul_rn(a.low, a.k), 0.f};
         bool wide = false;
         Batches x;
         Terms t;
@@ -679,16 +691,20 @@ __global__ void __launch_bounds__(256) preference_pairs_kernel(int pairs, const 
     }
 }
 
-// Threads of a row by the bytes of its logits: a warp up to 4 KB, 128 up to 32 KB, kRowThreads above, so that each has several vectors.
-int row_threads(const wkv6_token_logits *p) {
-    const int64_t n = (int64_t)p->V * (int64_t)dtype_size(p->dtype);
-    return n <= 4096 ? 32 : n <= 32768 ? 128 : kRowThreads;
+// Threads of a row by the bytes of its logits.  A warp saves the block's barriers: up to 16 KB forward (100 M bf16 logits in rows of 8192:
+// policy loss 103 us, 116 with 128 threads; in rows of 12000: 108 and 105), up to 8 KB for the gradient alone (rows of 4096: 69 and 77 us; of
+// 8192: 71 and 65) - where there are rows enough for 32 warps on every SM, otherwise up to 4 KB.  128 threads up to 32 KB (rows of 16384:
+// 100 us, 107 with 256; of 32768: 97 and 95).
+int row_threads(const wkv6_token_logits *p, bool gradient) {
+    const int64_t n = (int64_t)p->V * (int64_t)dtype_size(p->dtype), rows = (int64_t)p->S * p->T;
+    const int64_t warp = rows < 32 * (int64_t)sm_count() ? 4096 : gradient ? 8192 : 16384;
+    return n <= warp ? 32 : n <= 32768 ? 128 : kRowThreads;
 }
 
 // f(std::integral_constant<int, THREADS>, T *) for the call's type and row size
 template <typename F>
-int dispatch(const wkv6_token_logits *p, F f) {
-    const int threads = row_threads(p);
+int dispatch(const wkv6_token_logits *p, bool gradient, F f) {
+    const int threads = row_threads(p, gradient);
     auto typed = [&](auto *t) {
         if (threads == 32) return f(std::integral_constant<int, 32>{}, t);
         if (threads == 128) return f(std::integral_constant<int, 128>{}, t);
@@ -725,7 +741,7 @@ int rows_of(const wkv6_token_logits *p, Rows *a, const char *what, bool need_log
 template <bool POLICY>
 int launch_rows(const wkv6_token_logits *p, const Rows &a, float *lp, float2 *stat, const Policy &q, float *coefficient, void *g,
                 cudaStream_t st) {
-    return dispatch(p, [&](auto size, auto *t) {
+    return dispatch(p, false, [&](auto size, auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int threads = size.value;
         const unsigned grid = (unsigned)(threads == 32 ? (a.rows + kWarpRows - 1) / kWarpRows : a.rows);
@@ -762,7 +778,7 @@ extern "C" int wkv6_token_log_probs_backward(const wkv6_token_logits *p, const f
     if (!stat || !coefficient || !g || (unless_one && !factor)) return fail(WKV6_ERR_INVALID, "wkv6_token_log_probs_backward: NULL argument");
     if (!aligned16(g) || reinterpret_cast<uintptr_t>(stat) % 8)
         return fail(WKV6_ERR_INVALID, "wkv6_token_log_probs_backward: the gradient must be 16-byte aligned, stat 8-byte");
-    return dispatch(p, [&](auto size, auto *t) {
+    return dispatch(p, true, [&](auto size, auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int threads = size.value;
         // parts of at least one stage, as many as it takes to give every SM its blocks

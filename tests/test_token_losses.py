@@ -203,6 +203,26 @@ def test_rows_that_do_not_count_are_not_read(V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [9, 300, 3000, 9000, 20000, 70001])
+def test_one_possible_token(V):
+    """All logits but one are -inf or the lowest value, wherever that one lies: its log-probability is 0, the others' gradient zero."""
+    from star_rwkv6_b200.loss import policy_loss, token_log_probs
+    at = sorted({0, 1, V // 3, V - 2, V - 1})
+    for none in (float("-inf"), torch.finfo(torch.bfloat16).min):
+        for tau in (0.3, 1.0, 7.0):
+            z = torch.full((1, len(at), V), none, device="cuda", dtype=torch.bfloat16)
+            t = torch.tensor([at], device="cuda")
+            z.scatter_(-1, t[..., None], 1.5)
+            z.requires_grad_(True)
+            one = torch.ones(1, len(at), device="cuda")
+            lp = token_log_probs(z, t, temperature=tau)
+            loss, again = policy_loss(z, t, one, 0 * one, temperature=tau)
+            assert (lp.abs() <= LP).all() and (again.abs() <= LP).all() and abs(loss.item() + 1) <= 4 * LP
+            g, h = torch.autograd.grad(lp, z, one)[0], torch.autograd.grad(loss, z)[0]
+            assert g.abs().max() <= LP / tau and h.abs().max() <= LP / tau
+
+
+@pytest.mark.gpu
 def test_rows_without_a_distribution_give_nan():
     from star_rwkv6_b200.loss import policy_loss, token_log_probs
     for V in (40, 5000):
