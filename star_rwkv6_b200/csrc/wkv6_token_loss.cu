@@ -413,27 +413,28 @@ struct Policy {
     int reduction;
     const int *counts;       // live rows of each part
     int parts;
-    float *row_loss;
+    float *row_loss;         // of each block
     unsigned *done;
     float *loss;
 };
 
-constexpr int kCountRows = 1024;    // rows of a part where tokens are counted over all sequences
+// Rows of a part where tokens are counted over all sequences: at most 64 parts, which every row adds up.
+__host__ __device__ constexpr int64_t count_rows(int64_t rows) { return rows > 64 * 1024 ? (rows + 63) / 64 : 1024; }
 constexpr int kWarpRows = 8;
 
-// The last block to draw a number behind its rows' losses adds up all rows, in an order that does not depend on which block that is.
+// The last block to draw a number behind its loss adds up all blocks', in an order that does not depend on which block that is.
 // Thread 0 draws it while the gradient is still to be written.
 __device__ __forceinline__ void draw_number(const Policy &q, bool &last) {
     __threadfence();
     last = atomicAdd(q.done, 1u) == gridDim.x - 1;
 }
-__device__ __forceinline__ void total_loss(const Policy &q, int64_t rows, const bool &last) {
+__device__ __forceinline__ void total_loss(const Policy &q, const bool &last) {
     __shared__ double part[32];
     __syncthreads();
     if (!last) return;
     __threadfence();
     double x = 0.0;
-    for (int64_t i = threadIdx.x; i < rows; i += blockDim.x) x += (double)__ldcg(q.row_loss + i);
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += blockDim.x) x += (double)__ldcg(q.row_loss + i);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = x;
@@ -512,6 +513,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, row_
 token_rows_kernel(const Rows a, float *__restrict__ lp_out, float2 *__restrict__ stat, const Policy q, float *__restrict__ coefficient,
                   T *__restrict__ g) {
     __shared__ bool last;
+    __shared__ float of_warp[kWarpRows];
     const int tid = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x;
     const int64_t row = THREADS == 32 ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
     if (THREADS != 32 || row < a.rows) {
@@ -538,9 +540,13 @@ token_rows_kernel(const Rows a, float *__restrict__ lp_out, float2 *__restrict__
             lp_out[row] = lp;
             if (stat != nullptr) stat[row] = make_float2(r.c, wide ? -inv_sum : inv_sum);
             if constexpr (POLICY) {
-                q.row_loss[row] = loss.x;
                 coefficient[row] = loss.y;
-                if (THREADS != 32) draw_number(q, last);
+                if (THREADS != 32) {
+                    q.row_loss[row] = loss.x;
+                    draw_number(q, last);
+                } else {
+                    of_warp[threadIdx.x >> 5] = loss.x;
+                }
             }
         }
         if constexpr (POLICY) {
@@ -562,11 +568,17 @@ token_rows_kernel(const Rows a, float *__restrict__ lp_out, float2 *__restrict__
         }
     }
     if constexpr (POLICY) {
-        if (THREADS == 32) {
+        if constexpr (THREADS == 32) {
             __syncthreads();
-            if (threadIdx.x == 0) draw_number(q, last);
+            if (threadIdx.x == 0) {
+                float x = 0.f;
+                for (int i = 0; i < kWarpRows; ++i)
+                    if (blockIdx.x * (int64_t)kWarpRows + i < a.rows) x += of_warp[i];
+                q.row_loss[blockIdx.x] = x;
+                draw_number(q, last);
+            }
         }
-        total_loss(q, a.rows, last);
+        total_loss(q, last);
     }
 }
 
@@ -612,7 +624,7 @@ token_gradient_kernel(const Rows a, const float2 *__restrict__ stat, const float
     }
 }
 
-// Live rows of every part: a sequence, or kCountRows rows of the whole where only their total is wanted.
+// Live rows of every part: a sequence, or count_rows() rows of the whole where only their total is wanted.
 __global__ void __launch_bounds__(256) count_rows_kernel(const Rows a, int64_t part_rows, int *__restrict__ counts, unsigned *__restrict__ done) {
     __shared__ int part[8];
     if (blockIdx.x == 0 && threadIdx.x == 0) *done = 0u;
@@ -752,7 +764,7 @@ int launch_rows(const wkv6_token_logits *p, const Rows &a, float *lp, float2 *st
 }
 
 int64_t count_parts(int64_t S, int64_t T, int reduction) {
-    return reduction == WKV6_SEQUENCE_MEAN ? S : (S * T + kCountRows - 1) / kCountRows;
+    return reduction == WKV6_SEQUENCE_MEAN ? S : (S * T + count_rows(S * T) - 1) / count_rows(S * T);
 }
 
 }  // namespace
@@ -835,7 +847,7 @@ extern "C" int wkv6_policy_loss(const wkv6_token_logits *p, const wkv6_policy *c
     q.counts = counts;
     q.parts = (int)count_parts(p->S, p->T, c->reduction);
     q.loss = loss;
-    count_rows_kernel<<<q.parts, 256, 0, st>>>(a, c->reduction == WKV6_SEQUENCE_MEAN ? p->T : kCountRows, counts, q.done);
+    count_rows_kernel<<<q.parts, 256, 0, st>>>(a, c->reduction == WKV6_SEQUENCE_MEAN ? p->T : count_rows(a.rows), counts, q.done);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "count_rows_kernel launch");
     return launch_rows<true>(p, a, log_probs, reinterpret_cast<float2 *>(stat), q, coefficient, g, st);
