@@ -1,6 +1,6 @@
 // AdamW over many tensors at once (include/wkv6_b200.h gives the formulas), states in fp32 or in blocks of 256 e4m3 codes with a scale.
 //
-// A bf16 value with fp32 states moves 22 bytes, with 8-bit states 10.06.  The first is bound by HBM: 368 M values (two layers, embedding
+// A bf16 value with fp32 states moves 22 bytes, with 8-bit states 10.06.  The first is bound by HBM: 379 M values (two layers, embedding
 // and head of the 1.6B shape) in 1328 us, 96 % of the copy bandwidth.  The second is bound by instructions: 896 us, 65 % of it, at 64.6
 // instructions per value (at the copy bandwidth there is time for 55): random bits, two square roots' and two conversions' worth of
 // work per value, and moments that keep the bits of elementary operations.
@@ -21,7 +21,7 @@ namespace wkv6 {
 
 namespace {
 
-// Two blocks per SM: with the next chunk's values in registers a thread needs 112 to 118 of them.  Measured for 368 M bf16 values: fp32
+// Two blocks per SM: with the next chunk's values in registers a thread needs 112 to 118 of them.  Measured for 379 M bf16 values: fp32
 // states 1328 us (three blocks 1519, four 1602); 8 bits 896 us with 16 values per thread and chunk (eight: 1017; not requested ahead: 983).
 constexpr int kThreads = 256, kPerThread = 8, kGroupValues = kThreads * kPerThread, kBlock = 256, kBlocksPerSm = 2;
 __host__ __device__ constexpr int groups(int bits) { return bits == 8 ? 2 : 1; }     // of eight values per thread and chunk
