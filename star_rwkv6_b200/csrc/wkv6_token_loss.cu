@@ -640,68 +640,107 @@ __global__ void __launch_bounds__(256) count_rows_kernel(const Rows a, int64_t p
     }
 }
 
-// log-probability of every sequence: its live rows' sum (in 64 bits: thousands of terms, of which only the difference to a
-// reference matters) or mean.  A block per sequence.
-__global__ void __launch_bounds__(256) sequence_sum_kernel(const Rows a, const float *__restrict__ lp, int average, float *__restrict__ seq,
-                                                           double *__restrict__ seq64, int *__restrict__ count) {
-    __shared__ double part[8];
-    __shared__ int live[8];
-    const int64_t first = (int64_t)blockIdx.x * a.T;
+// What the preference loss takes beside the rows.
+struct Pairs {
+    const float *lp, *ref;
+    double beta, smoothing, margin, scale;
+    int S, average;
+    float *seq;          // log-probability of every sequence
+    double *seq64;
+    int *count;          // of its live rows
+    float *coefficient, *loss;
+};
+
+// Log-probability of a sequence: its live rows' sum (in 64 bits: thousands of terms, of which only the difference to a
+// reference matters) or mean, by WARPS warps.
+template <int WARPS>
+__device__ __forceinline__ void sum_sequence(const Rows &a, const Pairs &q, int s) {
+    constexpr int THREADS = WARPS * 32, U = 8;
+    const int64_t first = (int64_t)s * a.T;
+    const int lane = threadIdx.x & 31, tid = WARPS == 1 ? lane : threadIdx.x;
     double x = 0.0;
     int n = 0;
-    for (int i = threadIdx.x; i < a.T; i += 256) {
-        if (target_of(a, first + i) >= 0) {
-            x += (double)lp[first + i];
-            ++n;
+    for (int i0 = tid; i0 < a.T; i0 += THREADS * U) {
+        float lp[U];
+        int target[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {      // requested together: those behind the end ask for the last one again
+            const int i = min(i0 + u * THREADS, a.T - 1);
+            lp[u] = q.lp[first + i];
+            target[u] = target_of(a, first + i);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool live = target[u] >= 0 && i0 + u * THREADS < a.T;
+            x += live ? (double)lp[u] : 0.0;
+            n += live;
         }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     n = __reduce_add_sync(0xffffffffu, n);
-    if ((threadIdx.x & 31) == 0) {
-        part[threadIdx.x >> 5] = x;
-        live[threadIdx.x >> 5] = n;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 8; ++i) {
-            x += part[i];
-            n += live[i];
+    if constexpr (WARPS > 1) {
+        __shared__ double part[WARPS];
+        __shared__ int live[WARPS];
+        if (lane == 0) {
+            part[threadIdx.x >> 5] = x;
+            live[threadIdx.x >> 5] = n;
         }
-        if (average && n > 1) x /= n;
-        seq64[blockIdx.x] = x;
-        seq[blockIdx.x] = (float)x;
-        count[blockIdx.x] = n;
+        __syncthreads();
+        if (threadIdx.x == 0)
+            for (int i = 1; i < WARPS; ++i) {
+                x += part[i];
+                n += live[i];
+            }
+    }
+    if (tid == 0) {
+        if (q.average && n > 1) x /= n;
+        q.seq64[s] = x;
+        q.seq[s] = (float)x;
+        q.count[s] = n;
     }
 }
 
 // One block: margin, loss and slope of every pair, their mean in a fixed order.
-__global__ void __launch_bounds__(256) preference_pairs_kernel(int pairs, const double *__restrict__ seq64, const int *__restrict__ count,
-                                                               const float *__restrict__ ref, double beta, double smoothing, double margin,
-                                                               int average, double scale, float *__restrict__ coefficient,
-                                                               float *__restrict__ loss) {
-    __shared__ double part[8];
+constexpr int kPairThreads = 256;
+__device__ __forceinline__ void all_pairs(const Pairs &q) {
+    __shared__ double part[kPairThreads / 32];
+    const int pairs = q.S / 2;
     double total = 0.0;
-    for (int i = threadIdx.x; i < pairs; i += 256) {
-        const int j = i + pairs;
-        double over = seq64[i] - seq64[j];
-        if (ref != nullptr) over -= (double)ref[i] - (double)ref[j];
-        const double d = beta * over - margin, tail = log1p(exp(-fabs(d)));
-        total += (1.0 - smoothing) * (tail + fmax(-d, 0.0));           // a NaN reaches the sum through the tail
-        if (smoothing != 0.0) total += smoothing * (tail + fmax(d, 0.0));
-        const double slope = -beta * (1.0 - smoothing - 1.0 / (1.0 + exp(-d))) * (scale / pairs);
-        coefficient[i] = (float)(slope / (average && count[i] > 1 ? count[i] : 1));
-        coefficient[j] = (float)(-slope / (average && count[j] > 1 ? count[j] : 1));
-    }
+    if (threadIdx.x < kPairThreads) {
+        for (int i = threadIdx.x; i < pairs; i += kPairThreads) {
+            const int j = i + pairs;
+            double over = q.seq64[i] - q.seq64[j];
+            if (q.ref != nullptr) over -= (double)q.ref[i] - (double)q.ref[j];
+            const double d = q.beta * over - q.margin, tail = log1p(exp(-fabs(d)));
+            total += (1.0 - q.smoothing) * (tail + fmax(-d, 0.0));           // a NaN reaches the sum through the tail
+            if (q.smoothing != 0.0) total += q.smoothing * (tail + fmax(d, 0.0));
+            const double slope = -q.beta * (1.0 - q.smoothing - 1.0 / (1.0 + exp(-d))) * (q.scale / pairs);
+            q.coefficient[i] = (float)(slope / (q.average && q.count[i] > 1 ? q.count[i] : 1));
+            q.coefficient[j] = (float)(-slope / (q.average && q.count[j] > 1 ? q.count[j] : 1));
+        }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = total;
+        for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = total;
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < 8; ++i) total += part[i];
-        *loss = (float)(total * (scale / pairs));
+        for (int i = 1; i < kPairThreads / 32; ++i) total += part[i];
+        *q.loss = (float)(total * (q.scale / pairs));
     }
 }
+
+// Few tokens: everything in one block, a warp per sequence, which saves a launch (3 us of the host).
+constexpr int kOneBlock = 1024;
+__global__ void __launch_bounds__(kOneBlock) preference_kernel(const Rows a, const Pairs q) {
+    for (int s = threadIdx.x >> 5; s < q.S; s += kOneBlock / 32) sum_sequence<1>(a, q, s);
+    __syncthreads();
+    all_pairs(q);
+}
+
+// Many tokens: a block per sequence, then the pairs.
+__global__ void __launch_bounds__(256) sequence_sum_kernel(const Rows a, const Pairs q) { sum_sequence<8>(a, q, blockIdx.x); }
+__global__ void __launch_bounds__(kPairThreads) preference_pairs_kernel(const Pairs q) { all_pairs(q); }
 
 // Threads of a row by the bytes of its logits.  A warp saves the block's barriers: up to 16 KB forward (100 M bf16 logits in rows of 8192:
 // policy loss 103 us, 116 with 128 threads; in rows of 12000: 108 and 105), up to 8 KB for the gradient alone (rows of 4096: 69 and 77 us; of
@@ -872,13 +911,29 @@ extern "C" int wkv6_preference_loss(const wkv6_token_logits *p, const float *log
     if (workspace_bytes < wkv6_preference_loss_workspace_bytes(p->S))
         return fail(WKV6_ERR_WORKSPACE, "wkv6_preference_loss: workspace of %zu bytes, %zu are needed", workspace_bytes,
                     wkv6_preference_loss_workspace_bytes(p->S));
-    double *seq64 = static_cast<double *>(workspace);
-    int *count = reinterpret_cast<int *>(seq64 + p->S);
-    sequence_sum_kernel<<<p->S, 256, 0, st>>>(a, log_probs, c->average, sequence_log_probs, seq64, count);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return cuda_fail(e, "sequence_sum_kernel launch");
-    preference_pairs_kernel<<<1, 256, 0, st>>>(p->S / 2, seq64, count, c->ref_log_probs, c->beta, c->label_smoothing, c->margin, c->average,
-                                               c->scale, coefficient, loss);
-    e = cudaGetLastError();
+    Pairs q{};
+    q.lp = log_probs;
+    q.ref = c->ref_log_probs;
+    q.beta = c->beta;
+    q.smoothing = c->label_smoothing;
+    q.margin = c->margin;
+    q.scale = c->scale;
+    q.S = p->S;
+    q.average = c->average;
+    q.seq = sequence_log_probs;
+    q.seq64 = static_cast<double *>(workspace);
+    q.count = reinterpret_cast<int *>(q.seq64 + p->S);
+    q.coefficient = coefficient;
+    q.loss = loss;
+    // one block against two launches: 3.1 and 3.8 us at 2 x 65, 5.0 and 4.6 at 8 x 1024, 7.1 and 4.5 at 32 x 700, 9.3 and 4.5 at 128 x 64
+    if (p->S <= 32 && p->T <= 1024) {
+        preference_kernel<<<1, kOneBlock, 0, st>>>(a, q);
+    } else {
+        sequence_sum_kernel<<<p->S, 256, 0, st>>>(a, q);
+        const cudaError_t e = cudaGetLastError();
+        if (e != cudaSuccess) return cuda_fail(e, "sequence_sum_kernel launch");
+        preference_pairs_kernel<<<1, kPairThreads, 0, st>>>(q);
+    }
+    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? WKV6_OK : cuda_fail(e, "preference_pairs_kernel launch");
 }

@@ -105,8 +105,11 @@ variable_list once(Tensor g, size_t inputs, const char *what) {
     return out;
 }
 
-void gradient(const Rows &r, const Tensor &stat, const Tensor &coefficient, bool per_sequence, const Tensor &factor, bool unless_one, Tensor &g) {
-    ok(api.token_log_probs_backward(&r.p, ptr(stat), ptr(coefficient), per_sequence, ptr(factor), unless_one, g.data_ptr(), stream_of(g)));
+// One buffer holds what the backward of a loss needs of the rows: n coefficients, then the statistics at an 8-byte boundary.
+float *stat_of(const Tensor &kept, int64_t n) { return ptr(kept) + (n + 1) / 2 * 2; }
+
+void gradient(const Rows &r, const float *stat, const float *coefficient, bool per_sequence, const Tensor &factor, bool unless_one, Tensor &g) {
+    ok(api.token_log_probs_backward(&r.p, stat, coefficient, per_sequence, ptr(factor), unless_one, g.data_ptr(), stream_of(g)));
 }
 
 Rows rows_again(const variable_list &saved, double temperature) {
@@ -142,7 +145,8 @@ struct TokenLogProbs : public torch::autograd::Function<TokenLogProbs> {
             c10::cuda::CUDAGuard guard(s[0].device());
             const Rows r = rows_again(s, ctx->saved_data["temperature"].toDouble());
             g = empty_like_logits(s[0]);
-            gradient(r, s[3], dense_floats(grads[0]), false, Tensor(), false, g);
+            const Tensor coefficient = dense_floats(grads[0]);
+            gradient(r, ptr(s[3]), ptr(coefficient), false, Tensor(), false, g);
         }
         return once(g, 2, "the gradient of token_log_probs is not differentiable");
     }
@@ -156,21 +160,20 @@ struct PolicyCall {
     int32_t reduction = 0;
 };
 
+// kept: what the backward needs of the rows (the coefficients [rows], the statistics [rows, 2]), and behind it the workspace
 struct PolicyResult {
-    Tensor loss, lp, stat, coefficient, g;
+    Tensor loss, lp, kept, g;
 };
 
 PolicyResult policy(const Rows &r, const Tensor &targets, const PolicyCall &c, bool want_grad) {
     PolicyResult o;
+    const int64_t rows = r.S * r.T, held = (rows * 3 + 1 + 3) / 4 * 4;      // the workspace at a 16-byte boundary
     const size_t nbytes = api.policy_loss_workspace_bytes(r.p.S, r.p.T, c.reduction);
     o.loss = floats({}, r.z);
     o.lp = floats(targets.sizes(), r.z);
-    o.coefficient = floats({r.S * r.T}, r.z);
-    if (want_grad) {
-        o.stat = floats({r.S * r.T, 2}, r.z);
-        o.g = empty_like_logits(r.z);
-    }
-    Tensor ws = bytes(nbytes, r.z);
+    o.kept = floats({held + (int64_t)(nbytes + 3) / 4}, r.z);
+    if (want_grad) o.g = empty_like_logits(r.z);
+    float *coefficient = ptr(o.kept), *stat = stat_of(o.kept, rows);
     wkv6_policy q{};
     q.advantages = ptr(c.advantages);
     const int64_t d = c.advantages.dim();      // more than two: dense
@@ -183,8 +186,8 @@ PolicyResult policy(const Rows &r, const Tensor &targets, const PolicyCall &c, b
     q.kl_coef = c.kl;
     q.scale = c.scale;
     q.reduction = c.reduction;
-    ok(api.policy_loss(&r.p, &q, ptr(o.loss), ptr(o.lp), ptr(o.stat), ptr(o.coefficient), want_grad ? o.g.data_ptr() : nullptr, ws.data_ptr(),
-                       nbytes, stream_of(o.lp)));
+    ok(api.policy_loss(&r.p, &q, ptr(o.loss), ptr(o.lp), stat, coefficient, want_grad ? o.g.data_ptr() : nullptr, ptr(o.kept) + held, nbytes,
+                       stream_of(o.lp)));
     return o;
 }
 
@@ -195,7 +198,7 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
         Rows r;
         TORCH_CHECK(describe(logits, given, r), "wkv6: unsupported call");
         PolicyResult o = policy(r, given.targets, c, true);
-        ctx->save_for_backward({logits, r.targets, given.mask, o.stat, o.coefficient});
+        ctx->save_for_backward({logits, r.targets, given.mask, o.kept});
         ctx->saved_data["temperature"] = given.temperature;
         ctx->saved_data["g"] = o.g;
         ctx->mark_non_differentiable({o.lp});
@@ -220,7 +223,7 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
             } else {
                 g = empty_like_logits(s[0]);
             }
-            gradient(r, s[3], s[4], false, factor, first, g);
+            gradient(r, stat_of(s[3], r.S * r.T), ptr(s[3]), false, factor, first, g);
         }
         return once(g, 3, "the gradient of policy_loss is not differentiable");
     }
@@ -234,18 +237,21 @@ struct PreferenceCall {
     bool average = false;
 };
 
+// kept: the coefficients [S] and statistics [rows, 2], and behind them the rows' log-probabilities and the workspace
 struct PreferenceResult {
-    Tensor loss, seq, stat, coefficient;
+    Tensor loss, seq, kept;
 };
 
-PreferenceResult preference(const Rows &r, const Tensor &targets, const PreferenceCall &c, bool want_grad) {
+PreferenceResult preference(const Rows &r, const PreferenceCall &c, bool want_grad) {
     PreferenceResult o;
-    const Tensor lp = log_probs(r, targets, want_grad ? &o.stat : nullptr);
+    const int64_t rows = r.S * r.T, held = (r.S + 1) / 2 * 2 + rows * 2, more = held + (rows + 1) / 2 * 2;      // even: 8-byte boundaries
+    const size_t nbytes = api.preference_loss_workspace_bytes(r.p.S);
     o.loss = floats({}, r.z);
     o.seq = floats({r.S}, r.z);
-    o.coefficient = floats({r.S}, r.z);
-    const size_t nbytes = api.preference_loss_workspace_bytes(r.p.S);
-    Tensor ws = bytes(nbytes, r.z);
+    o.kept = floats({more + (int64_t)(nbytes + 3) / 4}, r.z);
+    float *coefficient = ptr(o.kept), *lp = coefficient + held;
+    void *stream = stream_of(o.seq);
+    ok(api.token_log_probs(&r.p, lp, want_grad ? stat_of(o.kept, r.S) : nullptr, stream));
     wkv6_preference q{};
     q.ref_log_probs = ptr(c.ref);
     q.beta = c.beta;
@@ -253,7 +259,7 @@ PreferenceResult preference(const Rows &r, const Tensor &targets, const Preferen
     q.margin = c.margin;
     q.scale = c.scale;
     q.average = c.average;
-    ok(api.preference_loss(&r.p, ptr(lp), &q, ptr(o.loss), ptr(o.seq), ptr(o.coefficient), ws.data_ptr(), nbytes, stream_of(lp)));
+    ok(api.preference_loss(&r.p, lp, &q, ptr(o.loss), ptr(o.seq), coefficient, coefficient + more, nbytes, stream));
     return o;
 }
 
@@ -261,8 +267,8 @@ struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
     static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Given &given, const PreferenceCall &c) {
         Rows r;
         TORCH_CHECK(describe(logits, given, r), "wkv6: unsupported call");
-        PreferenceResult o = preference(r, given.targets, c, true);
-        ctx->save_for_backward({logits, r.targets, given.mask, o.stat, o.coefficient});
+        PreferenceResult o = preference(r, c, true);
+        ctx->save_for_backward({logits, r.targets, given.mask, o.kept});
         ctx->mark_non_differentiable({o.seq});
         ctx->set_materialize_grads(false);
         return {o.loss, o.seq};
@@ -277,7 +283,7 @@ struct PreferenceLoss : public torch::autograd::Function<PreferenceLoss> {
             c10::cuda::CUDAGuard guard(s[0].device());
             const Rows r = rows_again(s, 1.0);
             g = empty_like_logits(s[0]);
-            gradient(r, s[3], s[4], true, dense_floats(grads[0]), false, g);
+            gradient(r, stat_of(s[3], r.S), ptr(s[3]), true, dense_floats(grads[0]), false, g);
         }
         return once(g, 3, "the gradient of preference_loss is not differentiable");
     }
@@ -417,7 +423,7 @@ PyObject *py_preference_loss(PyObject *, PyObject *const *args, Py_ssize_t n) {
             loss = out[0];
             seq = out[1];
         } else {
-            PreferenceResult o = preference(r, given.targets, c, false);
+            PreferenceResult o = preference(r, c, false);
             loss = o.loss;
             seq = o.seq;
         }
@@ -522,6 +528,7 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
         c.grad_scale = static_cast<const float *>(at_device);
     }
     std::vector<wkv6_adamw_tensor> table[2];       // bf16, fp32
+    for (auto &x : table) x.reserve(count);
     for (Py_ssize_t i = 0; i < count; ++i) {
         const int64_t size = p[i]->numel(), blocks = (size + 255) / 256;
         const at::ScalarType t = p[i]->scalar_type();

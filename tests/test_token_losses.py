@@ -118,7 +118,8 @@ def test_policy_loss(S, T, V, dtype, kl, tau, reduction):
 @pytest.mark.gpu
 @pytest.mark.parametrize("P,T,V,dtype,smoothing,average,reference,margin", [
     (1, 1, 5, "f32", 0.0, False, True, 0.0), (3, 7, 259, "bf16", 0.1, True, False, 0.5), (2, 300, 1000, "f32", 0.2, False, True, 0.0),
-    (2, 3, 65536, "bf16", 0.0, False, True, 0.0), (300, 2, 9, "f16", 0.0, True, True, 0.0)])
+    (2, 3, 65536, "bf16", 0.0, False, True, 0.0), (300, 2, 9, "f16", 0.0, True, True, 0.0), (2, 1031, 40, "f32", 0.0, False, True, 0.1),
+    (16, 300, 33, "bf16", 0.05, True, True, 0.0)])
 def test_preference_loss(P, T, V, dtype, smoothing, average, reference, margin):
     from star_rwkv6_b200.loss import preference_loss
     z, targets, mask, g = _inputs(2 * P, T, V, TYPES[dtype], seed=4)
