@@ -244,7 +244,7 @@ WKV6_API int wkv6_scale_bf16(int64_t n, void *g, const float *scale, void *strea
  * its gradient is zeros.  Gradients are dense [S, T, V] of `dtype` and must not overlap the logits.
  */
 typedef struct {
-    int32_t S, T, V;
+    int32_t S, T, V;                     /* S * T < 2^31, V <= 2^30 */
     int32_t dtype;                       /* logits and their gradient: WKV6_BF16, WKV6_F16, WKV6_F32; aligned to one element */
     float temperature;                   /* at least 1e-30 */
     int64_t seq_stride, row_stride;

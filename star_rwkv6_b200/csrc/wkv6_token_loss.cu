@@ -2,7 +2,7 @@
 // KL term and the loss of paired log ratios.  For every token (row) with logits z[V], target a, temperature tau, k = log2(e) / tau:
 //   c = k max z,   s = sum_j 2^(k z_j - c),   lp = (k z_a - c - log2 s) ln 2,   p_j = 2^(k z_j - c) / s
 //   d lp / d z_j = (1[j = a] - p_j) / tau
-// Everything is bound by the bytes of the logits (65536 of them per token), and next by instructions: at the copy bandwidth a bf16
+// Everything is bound by the bytes of the logits (65536 of them per token) and next by instructions: at the copy bandwidth a bf16
 // logit has to be done with in 11 (it takes 6.4 forward, 15 with the gradient behind it, for which there is twice the time).  A row's
 // maximum and sum are taken in one pass (the sum is rescaled when the maximum grows), and where the gradient needs nothing but the row
 // itself (policy loss) the row is gone through again right behind that, from its end to its start: the end is still in registers, the
@@ -325,8 +325,8 @@ __device__ __forceinline__ void row_gradient(const Share<T, THREADS> &w, Batches
     if (b == 0) put(0, x.odd);
 }
 
-// The same without shared memory: for rows of a few KB, for the wide way, and for logits that lie at another offset from the 16-byte
-// boundaries than the gradient (their values are loaded one by one).
+// The same for the wide way, and for logits that lie at another offset from the 16-byte boundaries than the gradient (their values are
+// loaded one by one).
 template <typename T, bool WIDE>
 __device__ __forceinline__ void row_gradient_direct(const T *z, T *out, const Cut &l, int target, float k, float c, float neg, float g, int first, int step) {
     constexpr int N = Vec<T>::N, U = 2;
@@ -488,6 +488,9 @@ __device__ __forceinline__ float2 loss_of(const Rows &a, const Policy &q, Terms 
     return make_float2(loss * w, slope * w);
 }
 
+// A log-probability that rounding has lifted above 0; a NaN stays.
+__device__ __forceinline__ float at_most_zero(float x) { return x > 0.f ? 0.f : x; }
+
 // From the threads' parts of a row to its log-probability: r becomes the row's (c and sum), `wide` says how.
 template <typename T, int THREADS>
 __device__ __forceinline__ float finish_row(const Rows &a, const T *z, float zt, int tid, Part &r, bool &wide) {
@@ -497,13 +500,13 @@ __device__ __forceinline__ float finish_row(const Rows &a, const T *z, float zt,
     if (wide) {
         row_part_wide(z, a.V, tid, THREADS, a.k, r.c, r.sum);
         gather<THREADS, 1>(r.c, r.sum, a.k);
-        return (zt - r.c) * a.inv_tau - logf(r.sum);
+        return at_most_zero((zt - r.c) * a.inv_tau - logf(r.sum));
     }
     // The logarithm's whole part is taken off first, which is exact or nearly so: only a part in [0, 1) is off by its rounding.  (r.sum is
     // at least about 1; the last term is 0, or NaN where the sum is.)
     const uint32_t bits = __float_as_uint(r.sum);
     const float whole = (float)((int)(bits >> 23) - 127), part = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
-    return ((fmaf(zt, a.k, -r.c) - whole) - log2f(part)) * 0.69314718055994531f + (r.sum - r.sum);
+    return at_most_zero(((fmaf(zt, a.k, -r.c) - whole) - log2f(part)) * 0.69314718055994531f + (r.sum - r.sum));
 }
 
 // THREADS = 32: a warp per row, several to a block (rows of a few KB, where a block's reduction would cost more than its row);
@@ -660,12 +663,12 @@ __device__ __forceinline__ void sum_sequence(const Rows &a, const Pairs &q, int 
     const int lane = threadIdx.x & 31, tid = WARPS == 1 ? lane : threadIdx.x;
     double x = 0.0;
     int n = 0;
-    for (int i0 = tid; i0 < a.T; i0 += THREADS * U) {
+    for (int64_t i0 = tid; i0 < a.T; i0 += THREADS * U) {
         float lp[U];
         int target[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {      // requested together: those behind the end ask for the last one again
-            const int i = min(i0 + u * THREADS, a.T - 1);
+            const int64_t at = i0 + u * THREADS, i = at < a.T ? at : a.T - 1;
             lp[u] = q.lp[first + i];
             target[u] = target_of(a, first + i);
         }
@@ -773,6 +776,7 @@ int rows_of(const wkv6_token_logits *p, Rows *a, const char *what, bool need_log
     if (!(p->temperature >= 1e-30f) || std::isinf(p->temperature)) return fail(WKV6_ERR_INVALID, "%s: temperature must be at least 1e-30 and finite", what);
     a->rows = (int64_t)p->S * p->T;
     if (a->rows > 2147483647LL) return fail(WKV6_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 tokens", what);
+    if (p->V > 1 << 30) return fail(WKV6_ERR_UNSUPPORTED, "%s: V=%d, at most 2^30", what, p->V);
     a->T = p->T;
     a->V = p->V;
     a->row_stride = p->row_stride ? p->row_stride : p->V;

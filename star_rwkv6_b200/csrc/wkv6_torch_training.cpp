@@ -56,7 +56,7 @@ bool describe(const Tensor &logits, const Given &given, Rows &r) {
     const int64_t d = logits.dim();
     if (d < 1 || targets.dim() != d - 1 || dtype_code(logits.scalar_type()) < 0 || targets.scalar_type() != at::kLong) return false;
     const int64_t V = logits.size(d - 1), rows = targets.numel();
-    if (V < 1 || V >= (1LL << 31) || rows < 1 || rows >= (1LL << 31)) return false;
+    if (V < 1 || V > (1LL << 30) || rows < 1 || rows >= (1LL << 31)) return false;
     if (!std::equal(targets.sizes().begin(), targets.sizes().end(), logits.sizes().begin()) || targets.device() != logits.device()) return false;
     if (mask.defined() && (mask.scalar_type() != at::kBool || mask.sizes() != targets.sizes() || mask.device() != logits.device())) return false;
     if (V > 1 && logits.stride(d - 1) != 1) return false;

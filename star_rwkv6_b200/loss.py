@@ -87,8 +87,8 @@ def _check_targets(logits, targets, mask, temperature):
             raise ValueError("logits, targets and mask must be on one device")
     if not (temperature >= 1e-30 and math.isfinite(temperature)):
         raise ValueError("temperature must be at least 1e-30 and finite")
-    if targets.numel() >= 2 ** 31 or logits.shape[-1] >= 2 ** 31:
-        raise ValueError("more than 2^31 - 1 tokens, or entries of the vocabulary")
+    if targets.numel() >= 2 ** 31 or logits.shape[-1] > 2 ** 30:
+        raise ValueError("more than 2^31 - 1 tokens, or 2^30 entries of the vocabulary")
 
 
 def _per_token(t, name, targets, strided=False):

@@ -218,7 +218,7 @@ def test_one_possible_token(V):
             one = torch.ones(1, len(at), device="cuda")
             lp = token_log_probs(z, t, temperature=tau)
             loss, again = policy_loss(z, t, one, 0 * one, temperature=tau)
-            assert (lp.abs() <= LP).all() and (again.abs() <= LP).all() and abs(loss.item() + 1) <= 4 * LP
+            assert (lp.abs() <= LP).all() and (again.abs() <= LP).all() and not (lp > 0).any() and abs(loss.item() + 1) <= 4 * LP
             g, h = torch.autograd.grad(lp, z, one)[0], torch.autograd.grad(loss, z)[0]
             assert g.abs().max() <= LP / tau and h.abs().max() <= LP / tau
 
@@ -497,6 +497,7 @@ def test_refusals_of_the_library():
                dict(row_stride=-8), dict(logits=a + 1)):
         assert lib.wkv6_token_log_probs(rows(**kw), a, None, None) == -1, kw
     assert lib.wkv6_token_log_probs(rows(S=70000, T=70000), a, None, None) == -2
+    assert lib.wkv6_token_log_probs(rows(V=(1 << 30) + 1), a, None, None) == -2
     assert lib.wkv6_token_log_probs(rows(), None, None, None) == -1
     assert lib.wkv6_token_log_probs(rows(), a, a + 4, None) == -1 and b"stat" in lib.wkv6_last_error()
     assert lib.wkv6_token_log_probs(rows(S=0, logits=0, targets=0), None, None, None) == 0
