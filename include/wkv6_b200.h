@@ -259,6 +259,9 @@ WKV6_API int wkv6_token_log_probs(const wkv6_token_logits *p, float *log_probs, 
  * (one fp32 value on the device) may be NULL.  unless_one: nothing is done where *factor is 1. */
 WKV6_API int wkv6_token_log_probs_backward(const wkv6_token_logits *p, const float *stat, const float *coefficient, int32_t per_sequence,
                                            const float *factor, int32_t unless_one, void *g, void *stream);
+/* The number of the capture that the stream is part of, 0 outside of one: what a replay of one graph writes is not current at a replay
+ * of another. */
+WKV6_API uint64_t wkv6_capture_id(void *stream);
 
 /* Clipped policy loss:  ratio = exp(lp - old),  d = ref - lp,
  *   loss = scale * sum of w * ( -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1) )

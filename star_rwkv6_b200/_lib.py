@@ -28,7 +28,7 @@ SYMBOLS = (
     "wkv6_shift_mix_forward", "wkv6_shift_mix_backward", "wkv6_shift_mix_workspace_bytes", "wkv6_shift_mix_pair_forward", "wkv6_shift_mix_pair_backward",
     "wkv6_lora_mix_forward", "wkv6_lora_mix_backward",
     "wkv6_token_log_probs", "wkv6_token_log_probs_backward", "wkv6_policy_loss", "wkv6_policy_loss_workspace_bytes",
-    "wkv6_preference_loss", "wkv6_preference_loss_workspace_bytes", "wkv6_adamw_step",
+    "wkv6_preference_loss", "wkv6_preference_loss_workspace_bytes", "wkv6_capture_id", "wkv6_adamw_step",
     "wkv6_layer_norm_forward", "wkv6_layer_norm_backward", "wkv6_layer_norm_workspace_bytes", "wkv6_copy_2d_async",
     "wkv6_relu_sq_forward", "wkv6_relu_sq_backward", "wkv6_sigmoid_mul_forward", "wkv6_sigmoid_mul_backward",
     "wkv6_xla_forward", "wkv6_xla_backward", "wkv6_xla_forward_with_state", "wkv6_xla_forward_ckpt", "wkv6_xla_backward_ws",
@@ -182,6 +182,8 @@ def _load():
     lib.wkv6_token_log_probs.argtypes = [rows, vp, vp, vp]
     lib.wkv6_token_log_probs_backward.restype = ctypes.c_int
     lib.wkv6_token_log_probs_backward.argtypes = [rows, vp, vp, i32, vp, i32, vp, vp]
+    lib.wkv6_capture_id.restype = ctypes.c_uint64
+    lib.wkv6_capture_id.argtypes = [vp]
     lib.wkv6_policy_loss_workspace_bytes.restype = sz
     lib.wkv6_policy_loss_workspace_bytes.argtypes = [i32] * 3
     lib.wkv6_policy_loss.restype = ctypes.c_int

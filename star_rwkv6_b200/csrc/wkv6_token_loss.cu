@@ -847,6 +847,16 @@ extern "C" int wkv6_token_log_probs_backward(const wkv6_token_logits *p, const f
     });
 }
 
+extern "C" uint64_t wkv6_capture_id(void *stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+        cudaGetLastError();      // the legacy stream next to a capture: it is not part of it
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
+
 extern "C" size_t wkv6_policy_loss_workspace_bytes(int32_t S, int32_t T, int32_t reduction) {
     if (S <= 0 || T <= 0) return 0;
     return 16 + (size_t)((int64_t)S * T) * 4 + (size_t)count_parts(S, T, reduction) * 4;

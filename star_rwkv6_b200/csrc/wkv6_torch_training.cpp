@@ -18,6 +18,7 @@ namespace {
 struct Api {
     decltype(&::wkv6_token_log_probs) token_log_probs = nullptr;
     decltype(&::wkv6_token_log_probs_backward) token_log_probs_backward = nullptr;
+    decltype(&::wkv6_capture_id) capture_id = nullptr;
     decltype(&::wkv6_policy_loss) policy_loss = nullptr;
     decltype(&::wkv6_policy_loss_workspace_bytes) policy_loss_workspace_bytes = nullptr;
     decltype(&::wkv6_preference_loss) preference_loss = nullptr;
@@ -191,8 +192,9 @@ PolicyResult policy(const Rows &r, const Tensor &targets, const PolicyCall &c, b
     return o;
 }
 
-// The forward leaves the gradient for a loss that is the end of the graph; for another factor, or a second backward, it is formed
-// anew from the logits (the first one belongs to whoever received it).
+// The forward leaves the gradient for a loss that is the end of the graph; for another factor, a second backward, or one that is
+// captured into a graph that the forward is not part of, it is formed anew from the logits (the first one belongs to whoever received
+// it, and a replay must not find it as the last one left it).
 struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
     static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Given &given, const PolicyCall &c) {
         Rows r;
@@ -201,6 +203,7 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
         ctx->save_for_backward({logits, r.targets, given.mask, o.kept});
         ctx->saved_data["temperature"] = given.temperature;
         ctx->saved_data["g"] = o.g;
+        ctx->saved_data["capture"] = (int64_t)api.capture_id(stream_of(o.lp));
         ctx->mark_non_differentiable({o.lp});
         ctx->set_materialize_grads(false);
         return {o.loss, o.lp};
@@ -216,13 +219,13 @@ struct PolicyLoss : public torch::autograd::Function<PolicyLoss> {
             const Rows r = rows_again(s, ctx->saved_data["temperature"].toDouble());
             const Tensor factor = dense_floats(grads[0]);
             auto kept = ctx->saved_data.find("g");
-            const bool first = kept != ctx->saved_data.end();
+            bool first = kept != ctx->saved_data.end();
             if (first) {
                 g = kept->second.toTensor();
                 ctx->saved_data.erase(kept);
-            } else {
-                g = empty_like_logits(s[0]);
+                first = (int64_t)api.capture_id(stream_of(g)) == ctx->saved_data["capture"].toInt();
             }
+            if (!first) g = empty_like_logits(s[0]);
             gradient(r, stat_of(s[3], r.S * r.T), ptr(s[3]), false, factor, first, g);
         }
         return once(g, 3, "the gradient of policy_loss is not differentiable");
@@ -555,6 +558,11 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
         if (!lists[k].empty()) add_spans(lists[k], spans);
     for (size_t i = 1; i < spans.size(); ++i)
         if (spans[i].begin < spans[i - 1].end) return none();
+    for (const Tensor *t : g) {      // gradients may share memory among themselves only
+        const uintptr_t a = reinterpret_cast<uintptr_t>(t->const_data_ptr()), b = a + t->nbytes();
+        const auto next = std::lower_bound(spans.begin(), spans.end(), Span{b, b});      // the first that begins at or behind its end
+        if (a < b && next != spans.begin() && (next - 1)->end > a) return none();
+    }
     {
         c10::cuda::CUDAGuard guard(dev);
         if (c.step_device == nullptr && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return none();
@@ -574,7 +582,7 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
 const char *bind_training(void *library) {
 #define SYM(name)                                                                                                                  \
     if ((api.name = reinterpret_cast<decltype(api.name)>(dlsym(library, "wkv6_" #name))) == nullptr) return "wkv6_" #name;
-    SYM(token_log_probs) SYM(token_log_probs_backward) SYM(policy_loss) SYM(policy_loss_workspace_bytes) SYM(preference_loss)
+    SYM(token_log_probs) SYM(token_log_probs_backward) SYM(capture_id) SYM(policy_loss) SYM(policy_loss_workspace_bytes) SYM(preference_loss)
     SYM(preference_loss_workspace_bytes) SYM(adamw_step) SYM(last_error)
 #undef SYM
     api.bound = true;

@@ -200,14 +200,15 @@ def _policy(logits, targets, mask, temperature, consts, numbers, reduction, want
 
 
 class _PolicyLoss(torch.autograd.Function):
-    """The forward leaves the gradient for a loss that is the end of the graph.  Where another factor arrives, or the backward runs
-    again, it is formed anew from the logits (the first one belongs to whoever received it)."""
+    """The forward leaves the gradient for a loss that is the end of the graph.  Where another factor arrives, the backward runs again,
+    or is captured into a CUDA graph that the forward is not part of, it is formed anew from the logits (the first one belongs to
+    whoever received it, and a replay must not find it as the last one left it)."""
 
     @staticmethod
     def forward(ctx, logits, targets, mask, temperature, consts, numbers, reduction):
         loss, lp, stat, coefficient, ctx.g = _policy(logits, targets, mask, temperature, consts, numbers, reduction, True)
         ctx.save_for_backward(logits, targets, mask, stat, coefficient)
-        ctx.temperature = temperature
+        ctx.temperature, ctx.capture = temperature, lib.wkv6_capture_id(_stream(lp.device))
         ctx.mark_non_differentiable(lp)
         ctx.set_materialize_grads(False)
         return loss, lp
@@ -218,6 +219,8 @@ class _PolicyLoss(torch.autograd.Function):
         if grad is None:
             return (None,) * 7
         g, ctx.g = ctx.g, None
+        if g is not None and lib.wkv6_capture_id(_stream(g.device)) != ctx.capture:
+            g = None
         g = _logit_gradient(ctx, ctx.saved_tensors[4], 0, grad.to(torch.float32), g is not None, g)
         return g, None, None, None, None, None, None
 

@@ -518,3 +518,44 @@ def test_refusals_of_the_library():
     assert lib.wkv6_preference_loss(rows(), a, q, a, a, a, a, 23, None) == -3
     assert lib.wkv6_preference_loss(rows(), None, q, a, a, a, a, 24, None) == -1
     assert ctypes.sizeof(L.TokenLogits) == 64 and ctypes.sizeof(L.Policy) == 80 and ctypes.sizeof(L.Preference) == 48
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_forward_and_backward_in_graphs_of_their_own(native, monkeypatch):
+    """The backward is replayed with several factors for one forward, and what received a gradient may write over it."""
+    import types
+    from star_rwkv6_b200 import loss as L
+    if not native:
+        monkeypatch.setattr(L, "_native", types.SimpleNamespace(policy_loss=lambda *a: None))
+    S, T, V = 3, 5, 900
+    z, targets, mask, g = _inputs(S, T, V, torch.bfloat16, seed=40)
+    static, targets, mask = z.cuda().requires_grad_(True), targets.cuda(), mask.cuda()
+    adv, old = torch.randn(S, T, generator=g).cuda(), torch.full((S, T), -6.5, device="cuda")
+    call = lambda: L.policy_loss(static, targets, adv, old, mask=mask)[0]
+    factor = torch.ones((), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            torch.autograd.grad(call(), static, factor)
+    torch.cuda.synchronize()
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(forward, stream=side):
+        loss = call()
+    with torch.cuda.graph(backward, stream=side, pool=forward.pool()):
+        (got,) = torch.autograd.grad(loss, static, factor)
+    torch.cuda.synchronize()
+    for k in range(2):
+        with torch.no_grad():
+            static.copy_(z.cuda() * (1 + k))
+        forward.replay()
+        for x in (1.0, 3.0, 1.0, 0.5, 1.0):
+            factor.fill_(x)
+            backward.replay()
+            eager = call()
+            torch.autograd.grad(eager, static, factor, retain_graph=True)
+            (want,) = torch.autograd.grad(eager, static, factor)       # the second one is formed from the logits, too
+            assert torch.equal(loss, eager) and torch.equal(got, want) and got.any()
+            got.zero_()
+    torch.cuda.synchronize()
