@@ -7,6 +7,7 @@ keeps the updates that are smaller than half a parameter's last bit on average, 
 """
 from __future__ import annotations
 
+import bisect
 import math
 
 import torch
@@ -17,10 +18,20 @@ from .ops import _DT, _check_cuda, _native, _ptr, _stream
 BLOCK = 256      # values that share a scale where states have 8 bits
 
 
-def _overlap(ts):
-    """Whether two of the tensors share memory."""
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in ts if t.numel())
-    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+def _spans(ts):
+    return sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in ts if t.numel())
+
+
+def _overlap(written, grads):
+    """Whether a tensor shares memory with one that is written.  Gradients may share it among themselves."""
+    spans = _spans(written)
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        return True
+    for a, b in _spans(grads):
+        i = bisect.bisect_left(spans, (b, b))          # the first that begins at or behind its end
+        if i and spans[i - 1][1] > a:
+            return True
+    return False
 
 
 def _check_lists(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales):
@@ -55,8 +66,8 @@ def _check_lists(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales):
                 raise ValueError("all tensors must be on one device")
             if l[i].layout != torch.strided or not l[i].is_contiguous():
                 raise ValueError(f"tensor {i} of a list is not contiguous")
-    if _overlap([t for l in lists if l is not grads for t in l]):
-        raise ValueError("parameters, moments and scales must not share memory")
+    if _overlap([t for l in lists if l is not grads for t in l], grads):
+        raise ValueError("parameters, moments and scales must not share memory, nor with gradients")
 
 
 def _device_value(t, dtype, name, dev):
@@ -194,7 +205,10 @@ class AdamW(torch.optim.Optimizer):
                 if len(batches) > 1:
                     raise RuntimeError("a capturable group's parameters must be on one device")
                 if group["step"] is None:
-                    group["step"] = torch.zeros((), dtype=torch.int64, device=next(iter(batches))[0])
+                    dev, at = next(iter(batches))
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("take a first step before the capture: a new step number would be set back at every replay")
+                    group["step"] = torch.full((), at, dtype=torch.int64, device=dev)
                 group["step"].add_(1)
             for (_, at), batch in batches.items():
                 ps, ss = [p for p, _ in batch], [s for _, s in batch]

@@ -410,3 +410,42 @@ def test_refusals_without_a_gpu():
     assert call(dtype=L.F16) == -2 and call(state_bits=16) == -2
     assert call(n=0, p=0) == 0 and call(count=0) == 0
     assert lib.wkv6_adamw_step(None, 0, None, None) == -1
+
+
+@pytest.mark.gpu
+def test_gradients_may_share_memory_among_themselves_only():
+    from star_rwkv6_b200.optim import adamw_step
+    f = lambda n: torch.zeros(n, device="cuda")
+    one, two = torch.ones(8, device="cuda"), f(24)
+    ps, qs = [f(8), f(5), f(0)], [f(8), f(5), f(0)]
+    states = [[f(len(p)) for p in ps] for _ in range(4)]
+    adamw_step(ps, [one, one[3:], one[:0]], states[0], states[1], step=1)
+    adamw_step(qs, [one.clone(), one[3:].clone(), f(0)], states[2], states[3], step=1)
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs)) and ps[0].all()
+    for p, g, m, v in ((two[:8], two[:8], f(8), f(8)), (two[:8], two[7:15], f(8), f(8)), (two[8:16], two[1:9], f(8), f(8)),
+                       (f(8), two[:8], two[4:12], f(8)), (f(8), two[:8], f(8), two[:8]), (f(24), two, two.new_zeros(24), two)):
+        with pytest.raises(ValueError, match="share memory"):
+            adamw_step([p], [g], [m], [v], step=1)
+    narrow = dict(dtype=torch.float8_e4m3fn, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        adamw_step([f(8)], [two[:8]], [torch.zeros(8, **narrow)], [torch.zeros(8, **narrow)], exp_avg_scales=[two[3:4]], exp_avg_sq_scales=[f(1)], step=1)
+    adamw_step([two[:8]], [two[8:16]], [f(8)], [two[16:]], step=1)      # side by side
+    assert not two.any()
+
+
+@pytest.mark.gpu
+def test_a_group_made_capturable_goes_on_from_its_step():
+    from star_rwkv6_b200.optim import AdamW
+    p, q = (torch.nn.Parameter(torch.ones(40, device="cuda")) for _ in range(2))
+    a, b = AdamW([p], lr=0.1), AdamW([q], lr=0.1)
+    for k in range(4):
+        p.grad = torch.full_like(p, 1.0 + k)
+        q.grad = p.grad.clone()
+        if k == 2:
+            a.param_groups[0]["capturable"] = True
+            with pytest.raises(RuntimeError, match="before the capture"):
+                with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                    a.step()
+        a.step()
+        b.step()
+    assert torch.equal(p, q) and int(a.param_groups[0]["step"]) == 4
