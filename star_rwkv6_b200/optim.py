@@ -89,8 +89,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp
     int would stay what it was).  ``lr``: a float, or one fp32 value on the device.
     ``grad_scale``: one fp32 value on the device that multiplies the gradients (clipping, loss scaling).
     ``stochastic_rounding``: bf16 parameters are rounded up or down with the probabilities that keep their mean, else to nearest.  The
-    random bits (also of 8-bit states) follow from ``seed``, the step, and the tensor's and the value's positions: the tensor's is
-    its place in the list plus ``first_index``."""
+    random bits (also of 8-bit states) follow from ``seed`` and the step (the lowest 32 bits of either), and the tensor's and the value's
+    positions: the tensor's is its place in the list plus ``first_index``."""
     params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
     m_scales = None if exp_avg_scales is None else list(exp_avg_scales)
     v_scales = None if exp_avg_sq_scales is None else list(exp_avg_sq_scales)

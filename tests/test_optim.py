@@ -449,3 +449,26 @@ def test_a_group_made_capturable_goes_on_from_its_step():
         a.step()
         b.step()
     assert torch.equal(p, q) and int(a.param_groups[0]["step"]) == 4
+
+
+@pytest.mark.gpu
+def test_a_tensor_of_more_than_32_bits():
+    """The last 700 values of a tensor of 2^32 + 700 (26 GB with its gradient and states); all others are zeros and stay so."""
+    l, tail, n = _make([700], (torch.bfloat16,), 8, seed=5), 700, 2 ** 32 + 700
+    seed, step, index = 77, 6, 0
+    big = {}
+    for key in ("p", "g", "m", "v"):
+        big[key] = [torch.zeros(n, dtype=l[key][0].dtype, device="cuda")]
+        big[key][0][-tail:] = l[key][0]
+    for key in ("ms", "vs"):
+        big[key] = [torch.zeros((n + 255) // 256, device="cuda")]
+        big[key][0][-3:] = l[key][0]
+    new, _, sizes = _oracle(l, 0, 8, step, seed, HYPER)
+    key = O.stir(np.uint64(index) ^ O.stir(np.uint64(step) ^ O.stir(np.uint64(seed))))
+    random = O.stir(np.arange(tail, dtype=np.uint64) ^ O.stir(key + np.uint64(1)))
+    _step(big, 8, step=step, seed=seed, **HYPER)
+    for key, count in (("p", tail), ("m", tail), ("v", tail), ("ms", 3), ("vs", 3)):
+        l[key][0].copy_(big[key][0][-count:])
+        for at in (0, 2 ** 31 // (n // len(big[key][0])), len(big[key][0]) - count - 1000):
+            assert not big[key][0][at:at + 1000].float().any()
+    _check(l, 0, 8, True, new, random, sizes)
