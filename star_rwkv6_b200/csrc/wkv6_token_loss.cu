@@ -6,12 +6,12 @@
 // logit has to be done with in 11 (it takes 6.4 forward, 15 with the gradient behind it, for which there is twice the time).  A row's
 // maximum and sum are taken in one pass (the sum is rescaled when the maximum grows), and where the gradient needs nothing but the row
 // itself (policy loss) the row is gone through again right behind that, from its end to its start: the end is still in registers, the
-// rest in the L2 cache.  A block of 256 threads has a row, four of them are on an SM: with 512 threads all warps of an SM compute or wait
+// start in shared memory, the middle in the L2 cache.  A block of 256 threads has a row, four of them are on an SM: with 512 threads all warps of an SM compute or wait
 // at once (rows of 65536 bf16: 80 us instead of 71 for 2968 of them), with 128 the rows under way do not fit the L2 cache (policy loss 415
 // us instead of 375), and rows that blocks claim and request ahead through shared memory took 92 us: more instructions, nothing gained.
 // Measured, 6000 rows of 65536 bf16, all of them counting: log-probabilities 121 us = 6.48 TB/s (99 % of the copy bandwidth), their
-// gradient 249 us = 6.31 TB/s, the policy loss with its gradient 301 us = 5.23 TB/s: its second pass comes from the L2 cache, which
-// loses about a fifth of the rows under way.
+// gradient 249 us = 6.31 TB/s, the policy loss with its gradient 281 us = 5.6 TB/s: what its second pass takes from the L2 cache is
+// lost there for 9 % of the rows (20 % without the part in shared memory, and 286 us).
 // Rows that the mask leaves out, or whose target is no token, are not read: their log-probability and gradient are zero
 // whatever the logits hold.
 // k z - c is one multiply-add: c is rounded, but it is the same c everywhere in a row, so that it cancels.  Logits near the end of the
@@ -269,18 +269,49 @@ struct Batches {
     uint4 even[kU], odd[kU];
 };
 
-// Maximum and sum over a thread's share of a row.  The last batch stays in x.odd, the one before it in x.even.
-template <typename T, int THREADS, bool KEEP>
-__device__ __forceinline__ void row_part(const Share<T, THREADS> &w, float k, Part &r, Batches &x) {
+// A thread's first batches of a row in shared memory, for a gradient right behind the row's sum (N = 0: none).  own: the thread's place,
+// which no other thread looks at.
+template <int THREADS, int N>
+struct Stash {
+    uint4 *own;       // NULL where no gradient follows
+    __device__ __forceinline__ void put(int b, const uint4 (&q)[kU]) const {
+        if constexpr (N > 0) {
+            if (own != nullptr && b < N) {
+#pragma unroll
+                for (int u = 0; u < kU; ++u) own[(b * kU + u) * THREADS] = q[u];
+            }
+        }
+    }
+    __device__ __forceinline__ bool get(int b, uint4 (&q)[kU]) const {
+        if constexpr (N > 0) {
+            if (b < N) {
+#pragma unroll
+                for (int u = 0; u < kU; ++u) q[u] = own[(b * kU + u) * THREADS];
+                return true;
+            }
+        }
+        return false;
+    }
+};
+
+// Maximum and sum over a thread's share of a row.  The last batch stays in x.odd, the one before it in x.even, and of those before them
+// the first ones in the stash.
+template <typename T, int THREADS, bool KEEP, int N>
+__device__ __forceinline__ void row_part(const Share<T, THREADS> &w, float k, Part &r, Batches &x, const Stash<THREADS, N> &stash) {
     const int n = w.batches();
     int b = n & 1;
     if (b) w.template load<KEEP>(0, x.odd);
     if (n > b) w.template load<KEEP>(b, x.even);
-    if (b) take<T, kU>(x.odd, k, r, w.count);          // where it is the only one, not all of it need be there
+    if (b) {
+        stash.put(0, x.odd);
+        take<T, kU>(x.odd, k, r, w.count);          // where it is the only one, not all of it need be there
+    }
     for (; b + 2 < n; b += 2) {
         w.template load<KEEP>(b + 1, x.odd);
+        stash.put(b, x.even);
         take<T, kU>(x.even, k, r);
         w.template load<KEEP>(b + 2, x.even);
+        stash.put(b + 1, x.odd);
         take<T, kU>(x.odd, k, r);
     }
     if (b < n) {
@@ -299,10 +330,10 @@ __device__ __forceinline__ void last_batches(const Share<T, THREADS> &w, Batches
 }
 
 // The gradient over a thread's share of a row, into out[0], out[THREADS], ..., from the end to the start: the end is in registers, what is
-// before it was read last.  own = the number of the thread's vector that holds the target (at place `at`), or -1.  STREAM: the gradient
+// before it was read last, and the start is in the stash.  own = the number of the thread's vector that holds the target (at place `at`), or -1.  STREAM: the gradient
 // is not to displace rows that are waiting for theirs in the second-level cache (387 us instead of 374 otherwise).
-template <typename T, int THREADS, bool STREAM>
-__device__ __forceinline__ void row_gradient(const Share<T, THREADS> &w, Batches &x, uint4 *out, int own, int at, float k, float c, float neg, float g) {
+template <typename T, int THREADS, bool STREAM, int N>
+__device__ __forceinline__ void row_gradient(const Share<T, THREADS> &w, Batches &x, const Stash<THREADS, N> &stash, uint4 *out, int own, int at, float k, float c, float neg, float g) {
     auto put = [&](int b, const uint4 (&q)[kU]) {
         uint4 *p = out + (int64_t)b * (kU * THREADS);
         const bool whole = (b + 1) * kU <= w.count;
@@ -318,9 +349,9 @@ __device__ __forceinline__ void row_gradient(const Share<T, THREADS> &w, Batches
     int b = w.batches() - 1;
     for (; b >= 1; b -= 2) {
         put(b, x.odd);
-        if (b >= 2) w.template load<false>(b - 2, x.odd);
+        if (b >= 2 && !stash.get(b - 2, x.odd)) w.template load<false>(b - 2, x.odd);
         put(b - 1, x.even);
-        if (b >= 3) w.template load<false>(b - 3, x.even);
+        if (b >= 3 && !stash.get(b - 3, x.even)) w.template load<false>(b - 3, x.even);
     }
     if (b == 0) put(0, x.odd);
 }
@@ -448,6 +479,19 @@ __device__ __forceinline__ void total_loss(const Policy &q, const bool &last) {
 constexpr int kRowThreads = 256;     // of a long row
 __host__ __device__ constexpr int row_blocks(int threads) { return 1024 / (threads == 32 ? 32 * kWarpRows : threads); }   // per SM
 
+// The policy loss of long rows keeps the first batches of a row in shared memory for the gradient: less is read from the L2 cache again,
+// and less of the rows under way has to last there.  Two batches (32 KB a block) of four blocks per SM, in fp32, which has fewer
+// instructions per byte to hide, three batches of three blocks: 6000 rows of 65536 bf16 279 us (286 without; 286 with three blocks of three
+// batches; 320 with four, which leave the first-level cache too little for the loads under way), of 32768 fp32 261 us (291 without, 279
+// with four blocks of two).  Rows of a warp or of 128 threads: nothing gained (16384 bf16: 97 us either way), short ones lose by it.
+template <typename T, int THREADS, bool POLICY>
+struct LongRows {
+    static constexpr bool kWide = sizeof(T) == 4;
+    static constexpr int kStash = POLICY && THREADS == kRowThreads ? (kWide ? 3 : 2) : 0;
+    static constexpr int kBlocks = kStash > 0 && kWide ? 3 : row_blocks(THREADS);
+    static constexpr int kBytes = kStash * kU * 16 * THREADS;
+};
+
 // What a row's loss takes beside its log-probability, requested before the row.
 struct Terms {
     float adv = 0.f, old = 0.f, ref = 0.f;
@@ -512,7 +556,7 @@ __device__ __forceinline__ float finish_row(const Rows &a, const T *z, float zt,
 // THREADS = 32: a warp per row, several to a block (rows of a few KB, where a block's reduction would cost more than its row);
 // otherwise a block per row.  POLICY: the loss and, with g, the gradient behind the log-probabilities.
 template <typename T, int THREADS, bool POLICY>
-__global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, row_blocks(THREADS))
+__global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, LongRows<T, THREADS, POLICY>::kBlocks)
 token_rows_kernel(const Rows a, float *__restrict__ lp_out, float2 *__restrict__ stat, const Policy q, float *__restrict__ coefficient,
                   T *__restrict__ g) {
     __shared__ bool last;
@@ -529,11 +573,13 @@ token_rows_kernel(const Rows a, float *__restrict__ lp_out, float2 *__restrict__
         Part r{a.low, __fmul_rn(a.low, a.k), 0.f};
         bool wide = false;
         Batches x;
+        extern __shared__ uint4 stashed[];
+        const Stash<THREADS, LongRows<T, THREADS, POLICY>::kStash> stash{g != nullptr ? stashed + tid : nullptr};
         Terms t;
         if constexpr (POLICY) t = terms_of(a, q, row);
         if (target >= 0) {
             const float zt = Vec<T>::get1(z[target]);
-            row_part<T, THREADS, POLICY>(share, a.k, r, x);
+            row_part<T, THREADS, POLICY>(share, a.k, r, x, stash);
             take_loose(z, l, tid, THREADS, a.k, r);
             lp = finish_row<T, THREADS>(a, z, zt, tid, r, wide);
             inv_sum = 1.f / r.sum;
@@ -562,7 +608,7 @@ token_rows_kernel(const Rows a, float *__restrict__ lp_out, float2 *__restrict__
                     row_gradient_direct<T, true>(z, gr, cut_of(gr, a.V), target, a.k, r.c, neg, gc, tid, THREADS);
                 } else if ((reinterpret_cast<uintptr_t>(z) - reinterpret_cast<uintptr_t>(gr)) % 16 == 0) {
                     const int at = target - l.head, vec = at / Vec<T>::N, own = at >= 0 && vec % THREADS == tid ? vec / THREADS : -1;
-                    row_gradient<T, THREADS, true>(share, x, reinterpret_cast<uint4 *>(gr + l.head) + tid, own, at % Vec<T>::N, a.k, r.c, neg, gc);
+                    row_gradient<T, THREADS, true>(share, x, stash, reinterpret_cast<uint4 *>(gr + l.head) + tid, own, at % Vec<T>::N, a.k, r.c, neg, gc);
                     gradient_loose<T, false>(z, gr, l, target, a.k, r.c, neg, gc, tid, THREADS);
                 } else {
                     row_gradient_direct<T, false>(z, gr, cut_of(gr, a.V), target, a.k, r.c, neg, gc, tid, THREADS);
@@ -619,7 +665,7 @@ token_gradient_kernel(const Rows a, const float2 *__restrict__ stat, const float
             const Share<T, THREADS> share(reinterpret_cast<const uint4 *>(z + l.head) + begin, n, tid);
             Batches x;
             last_batches(share, x);
-            row_gradient<T, THREADS, false>(share, x, reinterpret_cast<uint4 *>(gr + l.head) + begin + tid, own, at % Vec<T>::N, a.k, s.x, -gc * s.y, gc);
+            row_gradient<T, THREADS, false>(share, x, Stash<THREADS, 0>{nullptr}, reinterpret_cast<uint4 *>(gr + l.head) + begin + tid, own, at % Vec<T>::N, a.k, s.x, -gc * s.y, gc);
         }
         gradient_loose<T, false>(z, gr, l, target, a.k, s.x, -gc * s.y, gc, first, step);
     } else {
@@ -800,7 +846,12 @@ int launch_rows(const wkv6_token_logits *p, const Rows &a, float *lp, float2 *st
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int threads = size.value;
         const unsigned grid = (unsigned)(threads == 32 ? (a.rows + kWarpRows - 1) / kWarpRows : a.rows);
-        token_rows_kernel<T, threads, POLICY><<<grid, threads == 32 ? 32 * kWarpRows : threads, 0, st>>>(a, lp, stat, q, coefficient, static_cast<T *>(g));
+        const auto kernel = token_rows_kernel<T, threads, POLICY>;
+        const int stash = g != nullptr ? LongRows<T, threads, POLICY>::kBytes : 0;
+        if (stash >= 47 * 1024)      // with what the kernel declares, more than a launch may have unasked
+            if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, stash); e != cudaSuccess)
+                return cuda_fail(e, "cudaFuncSetAttribute");
+        kernel<<<grid, threads == 32 ? 32 * kWarpRows : threads, stash, st>>>(a, lp, stat, q, coefficient, static_cast<T *>(g));
         const cudaError_t e = cudaGetLastError();
         return e == cudaSuccess ? (int)WKV6_OK : cuda_fail(e, "token_rows_kernel launch");
     });
