@@ -7,8 +7,8 @@
 // maximum and sum are taken in one pass (the sum is rescaled when the maximum grows), and where the gradient needs nothing but the row
 // itself (policy loss) the row is gone through again right behind that, from its end to its start: the end is still in registers, the
 // start in shared memory, the middle in the L2 cache.  A block of 256 threads has a row, four of them are on an SM: with 512 threads all warps of an SM compute or wait
-// at once (rows of 65536 bf16: 80 us instead of 71 for 2968 of them), with 128 the rows under way do not fit the L2 cache (policy loss 415
-// us instead of 375), and rows that blocks claim and request ahead through shared memory took 92 us: more instructions, nothing gained.
+// at once (rows of 65536 bf16: 82 us instead of 72 for 2968 of them), with 128 the rows under way do not fit the L2 cache (policy loss of
+// 8192 such rows 418 us instead of 373), and rows that blocks claim and request ahead through shared memory took 92 us: more instructions, nothing gained.
 // Measured, 6000 rows of 65536 bf16, all of them counting: log-probabilities 121 us = 6.48 TB/s (99 % of the copy bandwidth), their
 // gradient 249 us = 6.31 TB/s, the policy loss with its gradient 281 us = 5.6 TB/s: what its second pass takes from the L2 cache is
 // lost there for 9 % of the rows (20 % without the part in shared memory, and 286 us).
@@ -233,7 +233,7 @@ __device__ __forceinline__ void gradient_loose(const T *z, T *out, const Cut &l,
 constexpr int kU = 4;         // vectors that a thread requests at once, while it computes on as many
 
 // Logits that are read once leave no line in the first-level cache; KEEP (the row will be read again): nor do the others, but with that
-// hint they also leave the second-level cache early (policy loss at 8192 x 65536: 340 MB read per 198 MB of rows, and 450 us for 392).
+// hint they also leave the second-level cache early (policy loss of 8192 rows of 65536 bf16: 402 us instead of 373).
 template <bool KEEP>
 __device__ __forceinline__ uint4 load16(const uint4 *p) {
     if (KEEP) return __ldg(p);
@@ -331,7 +331,7 @@ __device__ __forceinline__ void last_batches(const Share<T, THREADS> &w, Batches
 
 // The gradient over a thread's share of a row, into out[0], out[THREADS], ..., from the end to the start: the end is in registers, what is
 // before it was read last, and the start is in the stash.  own = the number of the thread's vector that holds the target (at place `at`), or -1.  STREAM: the gradient
-// is not to displace rows that are waiting for theirs in the second-level cache (387 us instead of 374 otherwise).
+// is not to displace rows that are waiting for theirs in the second-level cache (381 us instead of 373 otherwise).
 template <typename T, int THREADS, bool STREAM, int N>
 __device__ __forceinline__ void row_gradient(const Share<T, THREADS> &w, Batches &x, const Stash<THREADS, N> &stash, uint4 *out, int own, int at, float k, float c, float neg, float g) {
     auto put = [&](int b, const uint4 (&q)[kU]) {
@@ -481,7 +481,7 @@ __host__ __device__ constexpr int row_blocks(int threads) { return 1024 / (threa
 
 // The policy loss of long rows keeps the first batches of a row in shared memory for the gradient: less is read from the L2 cache again,
 // and less of the rows under way has to last there.  Two batches (32 KB a block) of four blocks per SM, in fp32, which has fewer
-// instructions per byte to hide, three batches of three blocks: 6000 rows of 65536 bf16 279 us (286 without; 286 with three blocks of three
+// instructions per byte to hide, three batches of three blocks: 6000 rows of 65536 bf16 281 us (287 without; 286 with three blocks of three
 // batches; 320 with four, which leave the first-level cache too little for the loads under way), of 32768 fp32 261 us (291 without, 279
 // with four blocks of two).  Rows of a warp or of 128 threads: nothing gained (16384 bf16: 97 us either way), short ones lose by it.
 template <typename T, int THREADS, bool POLICY>
