@@ -14,13 +14,16 @@
 // lost there for 9 % of the rows (20 % without the part in shared memory, and 286 us).
 // Rows that the mask leaves out, or whose target is no token, are not read: their log-probability and gradient are zero
 // whatever the logits hold.
-// k z - c is one multiply-add: c is rounded, but it is the same c everywhere in a row, so that it cancels.  Logits near the end of the
-// type's range, where k z overflows, take a second way (`wide`): their maximum is subtracted before the scaling.  A row of -inf has no
-// distribution and gives NaN.
+// k z - c is one multiply-add: c is rounded, but it is the same c everywhere in a part of a row, and what it is off by, as a power of two,
+// is a factor of that part's sum that the next rescaling takes off again.  It has to stay a harmless one: below |c| = 2^24 it is at most 2^(1/2).
+// Rows with a maximum beyond that (|z| / tau above 1.16e7) take a second way (`wide`), which subtracts the maximum before the scaling;
+// smaller logits among ordinary ones (fills of -1e10 and the like) lie below the maximum that every part starts with, and add zeros.
+// A row of -inf has no distribution and gives NaN.
 // The reference has no trainer (its trainer files are empty); these operators stand beside the next-token loss.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
@@ -41,7 +44,7 @@ struct Rows {
     int T, V;
     float k;         // log2(e) / tau
     float inv_tau;
-    float low;       // logits of larger magnitude, as a row's maximum, take the wide way: -FLT_MAX / 4 / max(k, 1)
+    float low;       // where a part's maximum starts; rows whose maximum is not between low and -low take the wide way
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -141,7 +144,8 @@ __device__ __forceinline__ float warp_sum(float x) {
     return x;
 }
 
-// What a part of a row has come to: its maximum (not below Rows::low, so that parts of nothing but -inf add zeros), c = k max, and the sum.
+// What a part of a row has come to: its maximum (not below Rows::low, so that parts of nothing but -inf or large fills add zeros), c = k max,
+// and the sum.
 struct Part {
     float mx, c, sum;
 };
@@ -539,7 +543,7 @@ __device__ __forceinline__ float at_most_zero(float x) { return x > 0.f ? 0.f : 
 template <typename T, int THREADS>
 __device__ __forceinline__ float finish_row(const Rows &a, const T *z, float zt, int tid, Part &r, bool &wide) {
     gather<THREADS, 0>(r.c, r.sum, 1.f);
-    const float end = -__fmul_rn(a.low, a.k);      // the same in all threads; a NaN in the sum stays what it is
+    const float end = -__fmul_rn(a.low, a.k);      // 2^24; the same in all threads; a NaN in the sum stays what it is
     wide = !(r.c > -end && r.c < end);
     if (wide) {
         row_part_wide(z, a.V, tid, THREADS, a.k, r.c, r.sum);
@@ -547,7 +551,7 @@ __device__ __forceinline__ float finish_row(const Rows &a, const T *z, float zt,
         return at_most_zero((zt - r.c) * a.inv_tau - logf(r.sum));
     }
     // The logarithm's whole part is taken off first, which is exact or nearly so: only a part in [0, 1) is off by its rounding.  (r.sum is
-    // at least about 1; the last term is 0, or NaN where the sum is.)
+    // at least about 2^(-1/2); the last term is 0, or NaN where the sum is.)
     const uint32_t bits = __float_as_uint(r.sum);
     const float whole = (float)((int)(bits >> 23) - 127), part = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
     return at_most_zero(((fmaf(zt, a.k, -r.c) - whole) - log2f(part)) * 0.69314718055994531f + (r.sum - r.sum));
@@ -835,7 +839,7 @@ int rows_of(const wkv6_token_logits *p, Rows *a, const char *what, bool need_log
     a->mask = p->mask;
     a->k = (float)(1.4426950408889634 / (double)p->temperature);
     a->inv_tau = (float)(1.0 / (double)p->temperature);
-    a->low = -FLT_MAX / 4.f / fmaxf(a->k, 1.f);
+    a->low = -(float)std::min(16777216.0 / (double)a->k, (double)FLT_MAX / 4.0);      // |c| < 2^24, see the top; no infinity for a tiny k
     return WKV6_OK;
 }
 
