@@ -548,13 +548,16 @@ __device__ __forceinline__ float finish_row(const Rows &a, const T *z, float zt,
     if (wide) {
         row_part_wide(z, a.V, tid, THREADS, a.k, r.c, r.sum);
         gather<THREADS, 1>(r.c, r.sum, a.k);
-        return at_most_zero((zt - r.c) * a.inv_tau - logf(r.sum));
+        const float below = zt - r.c;      // overflows between the ends of the type's range
+        return at_most_zero((below == -INFINITY ? zt * a.inv_tau - r.c * a.inv_tau : below * a.inv_tau) - logf(r.sum));
     }
+    const float below = fmaf(zt, a.k, -r.c);
+    if (below == -INFINITY) return zt * a.inv_tau + (r.sum - r.sum);      // the type's lowest value: its product with log2(e) leaves fp32, the rest is lost in it
     // The logarithm's whole part is taken off first, which is exact or nearly so: only a part in [0, 1) is off by its rounding.  (r.sum is
     // at least about 2^(-1/2); the last term is 0, or NaN where the sum is.)
     const uint32_t bits = __float_as_uint(r.sum);
     const float whole = (float)((int)(bits >> 23) - 127), part = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
-    return at_most_zero(((fmaf(zt, a.k, -r.c) - whole) - log2f(part)) * 0.69314718055994531f + (r.sum - r.sum));
+    return at_most_zero(((below - whole) - log2f(part)) * 0.69314718055994531f + (r.sum - r.sum));
 }
 
 // THREADS = 32: a warp per row, several to a block (rows of a few KB, where a block's reduction would cost more than its row);

@@ -130,3 +130,37 @@ def test_temperatures(tau, dtype):
         ok = (x.gather(-1, at[..., None])[..., 0] - x.amax(-1)).abs() < 1e38      # a log-probability that fp32 holds
         at = torch.where(ok, at, z.float().argmax(-1))
         _check(z, at, tau)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [40, 4099, 70001])
+def test_a_chosen_token_at_the_types_lowest_value(V, dtype):
+    """Masked with the type's lowest value, or another one whose product with log2(e) leaves fp32, and chosen all the same: the
+    log-probability is that value (temperature 1), infinite only where fp32 ends.  It must not turn a pair that holds it twice into NaN."""
+    from star_rwkv6_b200.loss import policy_loss, preference_loss, token_log_probs
+    dt = TYPES[dtype]
+    lowest = torch.finfo(dt).min
+    g = torch.Generator().manual_seed(V)
+    z = 3 * torch.randn(2, 4, V, generator=g).to(dt)
+    at = torch.randint(0, V, (2, 4), generator=g)
+    fills = torch.tensor([[lowest, 0.75 * lowest, 0.0, lowest], [0.75 * lowest, lowest, 0.0, lowest]]).to(dt)
+    z[:, [0, 1, 3]] = z[:, [0, 1, 3]].scatter(-1, at[:, [0, 1, 3], None], fills[:, [0, 1, 3], None])
+    z[:, 3] = z[:, 3].scatter(-1, (at[:, 3:] + 1) % V, -lowest / 2)        # half the type's range above zero
+    zc, t = z.cuda().requires_grad_(True), at.cuda()
+    for tau in (1.0, 2.0, 0.5):
+        lp, p, live = O.log_probs(_np(z), _np(at), None, tau)
+        lp = np.where(lp < -float(np.finfo(np.float32).max) * (1 + 2.0 ** -24), -np.inf, lp)
+        with np.errstate(invalid="ignore"):
+            _close(token_log_probs(zc, t, temperature=tau), lp, ABS + REL * np.abs(lp))
+        loss, got = policy_loss(zc, t, torch.ones(2, 4, device="cuda"), torch.zeros(2, 4, device="cuda"), temperature=tau)
+        with np.errstate(invalid="ignore"):
+            _close(got, lp, ABS + REL * np.abs(lp))
+        assert loss.isfinite() and torch.autograd.grad(loss, zc)[0].isfinite().all()
+    mask = torch.tensor([[True, False, True, False], [False, True, True, False]])
+    _, want_seq, want, c = O.preference(_np(z), _np(at), None, _np(mask))
+    loss, seq = preference_loss(zc, t, None, mask.cuda())
+    _close(seq, want_seq, 3 * ABS + REL * np.abs(want_seq))
+    (gz,) = torch.autograd.grad(loss, zc)
+    assert loss.isfinite() and gz.isfinite().all()
+    _gradient_close(gz, want, c[:, None], dt, 2.0 ** -22)        # |D| is above 1000: the slope is saturated
