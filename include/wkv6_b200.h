@@ -304,7 +304,8 @@ WKV6_API int wkv6_preference_loss(const wkv6_token_logits *p, const float *log_p
  * state_bits 32: m and v are fp32.  8: blocks of 256 values, counted from the tensor's first, share a scale (one fp32 value per block):
  * m = code * m_scale and sqrt(v) = code * v_scale with e4m3 codes, the scale 1/448 of the block's largest value; m is rounded to
  * nearest, sqrt(v) up or down with the probabilities that keep its mean (an optimizer step changes it by less than half an e4m3
- * step).  stochastic: bf16 parameters are rounded the same way, from 16 random bits each; otherwise to nearest.  The random bits are
+ * step; m changes by more of what it lacks, but a code whose gradients are gone falls only while beta1 is below 17/18, so that it may
+ * be at most 0.94 with 8 bits).  stochastic: bf16 parameters are rounded the same way, from 16 random bits each; otherwise to nearest.  The random bits are
  * a function of the lowest 32 bits of seed and t, the tensor's `index` and the value's place in it.
  * A gradient that is infinite or NaN makes its value NaN (8 bits: its block's moments too).
  * t is `step`, or *step_device where that is not NULL (at least 1); lr is `lr`, or *lr_device.  Tensors must not overlap; n == 0 is allowed.

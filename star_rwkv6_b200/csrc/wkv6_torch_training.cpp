@@ -500,6 +500,7 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (!numbers(args + 8, 4, x) || !(x[0] >= 0.0 && x[0] < 1.0 && x[1] >= 0.0 && x[1] < 1.0) || !(x[2] >= 0.0) || std::isinf(x[2]) || !std::isfinite(x[3]))
         return none();
     c.state_bits = narrow ? 8 : 32;
+    if (narrow && x[0] > 0.94) return none();
     c.beta1 = x[0];
     c.beta2 = x[1];
     c.eps = x[2];

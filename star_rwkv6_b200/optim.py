@@ -16,6 +16,12 @@ from ._lib import AdamWConfig, AdamWTensor, check, lib
 from .ops import _DT, _check_cuda, _native, _ptr, _stream
 
 BLOCK = 256      # values that share a scale where states have 8 bits
+BETA1 = 0.94     # the largest with 8 bits: above 17/18, first moments without gradients would never fall
+
+
+def _check_beta1(state_bits, beta1):
+    if state_bits == 8 and beta1 > BETA1:
+        raise ValueError(f"states in 8 bits take beta1 up to {BETA1}, not {beta1}: first moments are rounded to nearest and would not move")
 
 
 def _spans(ts):
@@ -84,7 +90,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp
 
     ``params``: bf16 or fp32, contiguous, both types in one list if need be; ``grads`` of their types.
     ``exp_avgs``, ``exp_avg_sqs``: fp32; or, with ``exp_avg_scales`` and ``exp_avg_sq_scales`` (fp32, one per 256 values counted from the
-    tensor's first), float8_e4m3fn codes: m = code * scale, sqrt(v) = code * scale.  New states are zeros in either form.
+    tensor's first), float8_e4m3fn codes: m = code * scale, sqrt(v) = code * scale.  New states are zeros in either form.  With 8 bits ``betas[0]`` is at most 0.94: m is rounded
+    to nearest, and what changes it by less than half a code's step (3 to 6 %) is lost.
     ``step``: t of this step, counted from 1; an int, or one int64 value on the device (a captured step reads it at every replay, an
     int would stay what it was).  ``lr``: a float, or one fp32 value on the device.
     ``grad_scale``: one fp32 value on the device that multiplies the gradients (clipping, loss scaling).
@@ -100,6 +107,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp
     _check_lists(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales)
     if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
         raise ValueError("betas must lie in [0, 1)")
+    _check_beta1(32 if m_scales is None else 8, betas[0])
     if not (math.isfinite(eps) and eps >= 0.0 and math.isfinite(weight_decay)):
         raise ValueError("eps must not be negative, eps and weight_decay must be finite")
     if not params:
@@ -147,7 +155,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp
 class AdamW(torch.optim.Optimizer):
     """AdamW over bf16 and fp32 parameters on CUDA devices, each group's in one launch per type (see ``adamw_step``).
 
-    ``state_bits``: 32 (fp32 moments) or 8 (e4m3 codes and a scale per 256 values).  ``stochastic_rounding``, ``seed``: how bf16
+    ``state_bits``: 32 (fp32 moments) or 8 (e4m3 codes and a scale per 256 values; ``betas[0]`` up to 0.94).  ``stochastic_rounding``, ``seed``: how bf16
     parameters are rounded.  ``lr`` may be a tensor (one fp32 value on the parameters' device).
     ``grad_scale``: an attribute, None or one fp32 value on the device that multiplies the gradients of the next steps.
     ``capturable``: the step number is kept on the device (one per group), so that ``step`` can be captured into a CUDA graph; every
@@ -167,6 +175,11 @@ class AdamW(torch.optim.Optimizer):
         self.grad_scale = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       stochastic_rounding=stochastic_rounding, seed=seed, capturable=capturable, step=None))
+
+    def add_param_group(self, param_group):
+        settings = {**self.defaults, **param_group}
+        _check_beta1(settings["state_bits"], settings["betas"][0])
+        super().add_param_group(param_group)
 
     def _state_of(self, p, group):
         s = self.state[p]
