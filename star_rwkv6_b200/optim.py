@@ -197,6 +197,17 @@ class AdamW(torch.optim.Optimizer):
             s["step"] = 0
         return s
 
+    @staticmethod
+    def _leave_capturable(group, state):
+        """A group that is capturable no longer goes on from its number on the device."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a group that is capturable no longer has to take its next step outside of the capture")
+        at = int(group["step"])
+        for p in group["params"]:
+            if state.get(p):
+                state[p]["step"] = at
+        group["step"] = None
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -205,6 +216,8 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         first = 0
         for group in self.param_groups:
+            if group["step"] is not None and not group["capturable"]:
+                self._leave_capturable(group, self.state)
             # parameters of one launch: on one device, and at one step (a parameter that had no gradient before is behind)
             batches = {}
             for p in group["params"]:

@@ -1,0 +1,49 @@
+"""Optimizer objects that are copied, saved, loaded and switched, and calls that fail half way: what they go on with."""
+import copy
+
+import pytest
+import torch
+
+
+def _pair(n=40, **kw):
+    from star_rwkv6_b200.optim import AdamW
+    ps = [torch.nn.Parameter(torch.linspace(-1, 1, n, device="cuda")) for _ in range(2)]
+    return ps, [AdamW([p], **kw) for p in ps]
+
+
+def _grad(ps, k):
+    for p in ps:
+        p.grad = torch.full_like(p, 1.0 + k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("before", [0, 2])
+def test_a_group_taken_out_of_capturable_goes_on_from_its_step(before):
+    """Bias corrections and random bits of step 5 and on, not those of the first step; and back again."""
+    (p, q), (a, b) = _pair(lr=0.1)
+    for k in range(10):
+        _grad((p, q), k % 3)
+        a.param_groups[0]["capturable"] = before <= k < 4 or k >= 7
+        if k == 4:
+            with pytest.raises(RuntimeError, match="outside of the capture"):
+                with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                    a.step()
+        a.step()
+        b.step()
+        assert torch.equal(p, q), k
+        if k in (5, 8):           # a copy goes on alike
+            r = torch.nn.Parameter(p.detach().clone())
+            c = type(a)([r], lr=0.1)
+            c.load_state_dict(a.state_dict())
+            assert c.param_groups[0]["capturable"] == (k == 8)
+            c.param_groups[0]["capturable"] = False
+            r.grad, q.grad = torch.ones_like(r), torch.ones_like(r)
+            d = copy.deepcopy(b.state_dict())
+            kept = q.detach().clone()
+            c.step()
+            b.step()
+            assert torch.equal(r, q)
+            b.load_state_dict(d)
+            with torch.no_grad():
+                q.copy_(kept)
+    assert a.state[p]["step"] == 7 and int(a.param_groups[0]["step"]) == 10
