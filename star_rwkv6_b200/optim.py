@@ -162,6 +162,8 @@ class AdamW(torch.optim.Optimizer):
     parameter that gets gradients must then get them from its group's first step on.  A float ``lr`` stays in a captured step as it was.
     ``state_dict`` holds the moments in their own types; ``load_state_dict`` keeps them (parameters do not lend them theirs)."""
 
+    grad_scale = None       # of the class: copies and unpickled optimizers do not go through __init__
+
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32,
                  stochastic_rounding: bool = True, seed: int = 0, capturable: bool = False):
         if state_bits not in (8, 32):
@@ -172,7 +174,6 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("betas must lie in [0, 1)")
         if not (math.isfinite(eps) and eps >= 0.0 and math.isfinite(weight_decay) and weight_decay >= 0.0):
             raise ValueError("eps and weight_decay must be finite and not negative")
-        self.grad_scale = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       stochastic_rounding=stochastic_rounding, seed=seed, capturable=capturable, step=None))
 

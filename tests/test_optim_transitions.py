@@ -1,5 +1,6 @@
 """Optimizer objects that are copied, saved, loaded and switched, and calls that fail half way: what they go on with."""
 import copy
+import pickle
 
 import pytest
 import torch
@@ -47,3 +48,26 @@ def test_a_group_taken_out_of_capturable_goes_on_from_its_step(before):
             with torch.no_grad():
                 q.copy_(kept)
     assert a.state[p]["step"] == 7 and int(a.param_groups[0]["step"]) == 10
+
+
+def test_copied_and_unpickled_optimizers_have_their_attributes():
+    from star_rwkv6_b200.optim import AdamW
+    opt = AdamW([torch.nn.Parameter(torch.zeros(4))])
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert other.grad_scale is None
+        other.step()
+
+
+@pytest.mark.gpu
+def test_copied_and_unpickled_optimizers_step():
+    for again in (copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))):
+        (p, _), (opt, _) = _pair(lr=0.1)
+        _grad((p,), 0)
+        opt.step()
+        other = again(opt)
+        q = other.param_groups[0]["params"][0]
+        assert q is not p and torch.equal(p, q)
+        _grad((p, q), 1)
+        opt.step()
+        other.step()
+        assert torch.equal(p, q) and other.state[q]["step"] == 2
