@@ -260,5 +260,6 @@ class AdamW(torch.optim.Optimizer):
             for key, x in state_dict["state"].get(i, {}).items():
                 self.state[p][key] = x.detach().to(p.device, copy=True) if isinstance(x, torch.Tensor) else x
         for group in self.param_groups:
-            if isinstance(group["step"], torch.Tensor) and group["params"]:
-                group["step"] = group["step"].to(group["params"][0].device, copy=True)
+            for key in ("step", "lr"):
+                if isinstance(group[key], torch.Tensor) and group["params"]:
+                    group[key] = group[key].to(group["params"][0].device, copy=True)

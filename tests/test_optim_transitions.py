@@ -71,3 +71,23 @@ def test_copied_and_unpickled_optimizers_step():
         opt.step()
         other.step()
         assert torch.equal(p, q) and other.state[q]["step"] == 2
+
+
+@pytest.mark.gpu
+def test_a_checkpoint_loaded_to_the_host(tmp_path):
+    """Learning rate and step number on the device, read back with map_location="cpu"."""
+    (p, q), (a, b) = _pair(lr=torch.full((), 0.1, device="cuda"), capturable=True)
+    _grad((p, q), 0)
+    a.step()
+    torch.save(a.state_dict(), tmp_path / "opt.pt")
+    saved = torch.load(tmp_path / "opt.pt", map_location="cpu")
+    assert saved["param_groups"][0]["lr"].device.type == "cpu"
+    b.load_state_dict(saved)
+    with torch.no_grad():
+        q.copy_(p)
+    _grad((p, q), 1)
+    a.step()
+    b.step()
+    assert torch.equal(p, q) and b.param_groups[0]["lr"].is_cuda
+    a.param_groups[0]["lr"].fill_(5.0)           # a copy, as the other values are
+    assert b.param_groups[0]["lr"].item() == torch.tensor(0.1).item() and saved["param_groups"][0]["lr"].device.type == "cpu"
