@@ -237,15 +237,20 @@ class AdamW(torch.optim.Optimizer):
                         raise RuntimeError("take a first step before the capture: a new step number would be set back at every replay")
                     group["step"] = torch.full((), at, dtype=torch.int64, device=dev)
                 group["step"].add_(1)
-            for (_, at), batch in batches.items():
+            for (_, at), batch in batches.items():      # one batch where the number is on the device
                 ps, ss = [p for p, _ in batch], [s for _, s in batch]
                 scales = ([s[k + "_scale"] for s in ss] for k in ("exp_avg", "exp_avg_sq")) if group["state_bits"] == 8 else (None, None)
                 m_scales, v_scales = scales
-                adamw_step(ps, [p.grad.contiguous() for p in ps], [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss],
-                           exp_avg_scales=m_scales, exp_avg_sq_scales=v_scales,
-                           step=group["step"] if group["capturable"] else at + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                           weight_decay=group["weight_decay"], seed=group["seed"], stochastic_rounding=group["stochastic_rounding"],
-                           grad_scale=self.grad_scale, first_index=first)
+                try:
+                    adamw_step(ps, [p.grad.contiguous() for p in ps], [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss],
+                               exp_avg_scales=m_scales, exp_avg_sq_scales=v_scales,
+                               step=group["step"] if group["capturable"] else at + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                               weight_decay=group["weight_decay"], seed=group["seed"], stochastic_rounding=group["stochastic_rounding"],
+                               grad_scale=self.grad_scale, first_index=first)
+                except Exception:
+                    if group["capturable"]:
+                        group["step"].sub_(1)      # refused: not a step
+                    raise
                 if not group["capturable"]:
                     for s in ss:
                         s["step"] = at + 1

@@ -91,3 +91,18 @@ def test_a_checkpoint_loaded_to_the_host(tmp_path):
     assert torch.equal(p, q) and b.param_groups[0]["lr"].is_cuda
     a.param_groups[0]["lr"].fill_(5.0)           # a copy, as the other values are
     assert b.param_groups[0]["lr"].item() == torch.tensor(0.1).item() and saved["param_groups"][0]["lr"].device.type == "cpu"
+
+
+@pytest.mark.gpu
+def test_a_refused_step_is_not_counted():
+    (p, q), (a, b) = _pair(lr=0.1, capturable=True)
+    for k in range(3):
+        _grad((p, q), k)
+        good = p.grad
+        p.grad = p.detach()                      # shares memory with what the step writes
+        with pytest.raises(ValueError, match="share memory"):
+            a.step()
+        p.grad = good
+        a.step()
+        b.step()
+        assert torch.equal(p, q) and int(a.param_groups[0]["step"]) == k + 1
