@@ -258,7 +258,17 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        super().load_state_dict(state_dict)
+        # between the hooks: behind those that make a state dict of another one, before those that look at what was loaded
+        seen = []
+        hooks = (self.register_load_state_dict_pre_hook(lambda _, d: seen.append(d)),
+                 self.register_load_state_dict_post_hook(lambda _: self._own_types(seen[0]), prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _own_types(self, state_dict):
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         own = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(saved, own):

@@ -106,3 +106,28 @@ def test_a_refused_step_is_not_counted():
         a.step()
         b.step()
         assert torch.equal(p, q) and int(a.param_groups[0]["step"]) == k + 1
+
+
+def test_hooks_of_loading():
+    """What a hook makes of a state dict is what is loaded, in the states' own types; hooks behind the loading see those."""
+    from star_rwkv6_b200.optim import AdamW
+    p, q = (torch.nn.Parameter(torch.zeros(300, dtype=torch.bfloat16)) for _ in range(2))
+    opt = AdamW([p, q])
+    group = {k: v for k, v in opt.param_groups[0].items() if k != "params"}
+    x = torch.arange(300.0) + 0.001
+    saved = {"state": {0: {"exp_avg": x, "exp_avg_sq": x, "step": 3}}, "param_groups": [dict(group, params=[0, 1])]}
+
+    def swap(optimizer, d):
+        return dict(d, state={1: dict(d["state"][0], step=4)})
+
+    def look(optimizer):
+        seen.append(optimizer.state[q]["exp_avg"].dtype)
+        optimizer.state[q]["exp_avg_sq"].zero_()
+
+    seen = []
+    opt.register_load_state_dict_pre_hook(swap)
+    opt.register_load_state_dict_post_hook(look)
+    opt.load_state_dict(saved)
+    s = opt.state[q]
+    assert seen == [torch.float32] and p not in opt.state and s["step"] == 4
+    assert torch.equal(s["exp_avg"], x) and s["exp_avg"] is not x and not s["exp_avg_sq"].any() and x.all()
