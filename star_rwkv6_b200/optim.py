@@ -112,6 +112,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp
         raise ValueError("eps must not be negative, eps and weight_decay must be finite")
     if not params:
         return
+    if not 0 <= first_index <= 2 ** 31 - len(params):
+        raise ValueError("a tensor's place in the list plus first_index must lie in [0, 2^31)")
     dev = params[0].device
     c = AdamWConfig()
     c.state_bits, c.stochastic, c.seed = 32 if m_scales is None else 8, bool(stochastic_rounding), seed
@@ -121,8 +123,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp
     else:
         if torch.cuda.is_current_stream_capturing():
             raise ValueError("a captured step needs its number on the device: an int would be the same at every replay")
-        if step < 1:
-            raise ValueError("steps are counted from 1")
+        if not 1 <= step < 2 ** 63:
+            raise ValueError("steps are counted from 1, in 64 bits")
         c.step = step
     if isinstance(lr, torch.Tensor):
         c.lr_device = _device_value(lr, torch.float32, "lr", dev)

@@ -131,3 +131,18 @@ def test_hooks_of_loading():
     s = opt.state[q]
     assert seen == [torch.float32] and p not in opt.state and s["step"] == 4
     assert torch.equal(s["exp_avg"], x) and s["exp_avg"] is not x and not s["exp_avg_sq"].any() and x.all()
+
+
+@pytest.mark.gpu
+def test_numbers_beyond_64_bits_are_refused():
+    from star_rwkv6_b200.optim import adamw_step
+    f = lambda: torch.zeros(8, device="cuda")
+    p = f()
+    for kw in (dict(step=2 ** 63), dict(step=2 ** 64 + 1), dict(step=1, first_index=-1), dict(step=1, first_index=2 ** 31),
+               dict(step=1, first_index=2 ** 64), dict(step=1, first_index=2 ** 31 - 1, more=True)):
+        ps = [p, f()] if kw.pop("more", False) else [p]
+        with pytest.raises(ValueError):
+            adamw_step(ps, [f() + 1 for _ in ps], [f() for _ in ps], [f() for _ in ps], **kw)
+    assert not p.any()
+    adamw_step([p], [f() + 1], [f()], [f()], step=2 ** 63 - 1, first_index=2 ** 31 - 1, seed=2 ** 70 + 5)
+    assert p.all()
