@@ -121,7 +121,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp
     if isinstance(step, torch.Tensor):
         c.step_device = _device_value(step, torch.int64, "step", dev)
     else:
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing(dev):
             raise ValueError("a captured step needs its number on the device: an int would be the same at every replay")
         if not 1 <= step < 2 ** 63:
             raise ValueError("steps are counted from 1, in 64 bits")
@@ -152,6 +152,11 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp
         for t in l:
             if not t.is_inference():
                 torch.autograd.graph.increment_version(t)
+
+
+def _capturing(dev):
+    with torch.cuda.device(dev):
+        return torch.cuda.is_current_stream_capturing()
 
 
 class AdamW(torch.optim.Optimizer):
@@ -189,7 +194,7 @@ class AdamW(torch.optim.Optimizer):
         if not s:
             if group["capturable"] and group["step"] is not None:
                 raise RuntimeError("a capturable group's parameters must have gradients from its first step on")
-            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            if p.is_cuda and _capturing(p.device):
                 raise RuntimeError("take a first step before the capture: new states would be zeroed at every replay")
             if group["state_bits"] == 32:
                 s["exp_avg"], s["exp_avg_sq"] = (torch.zeros(p.shape, dtype=torch.float32, device=p.device) for _ in range(2))
@@ -203,7 +208,7 @@ class AdamW(torch.optim.Optimizer):
     @staticmethod
     def _leave_capturable(group, state):
         """A group that is capturable no longer goes on from its number on the device."""
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing(group["step"].device):
             raise RuntimeError("a group that is capturable no longer has to take its next step outside of the capture")
         at = int(group["step"])
         for p in group["params"]:
@@ -235,7 +240,7 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError("a capturable group's parameters must be on one device")
                 if group["step"] is None:
                     dev, at = next(iter(batches))
-                    if torch.cuda.is_current_stream_capturing():
+                    if _capturing(dev):
                         raise RuntimeError("take a first step before the capture: a new step number would be set back at every replay")
                     group["step"] = torch.full((), at, dtype=torch.int64, device=dev)
                 group["step"].add_(1)

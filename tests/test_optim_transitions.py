@@ -146,3 +146,29 @@ def test_numbers_beyond_64_bits_are_refused():
     assert not p.any()
     adamw_step([p], [f() + 1], [f()], [f()], step=2 ** 63 - 1, first_index=2 ** 31 - 1, seed=2 ** 70 + 5)
     assert p.all()
+
+
+def test_the_capture_that_counts_is_the_parameters_devices(monkeypatch):
+    """Host logic on a stand-in for a second device: its stream is being captured, the current device's is not."""
+    from star_rwkv6_b200.optim import AdamW
+
+    class Parameter:
+        is_cuda, device, shape = True, torch.device("cuda:1"), (4,)
+
+    current = [torch.device("cuda:0")]
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = torch.device(dev)
+
+        def __enter__(self):
+            current.append(self.dev)
+
+        def __exit__(self, *args):
+            current.pop()
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: current[-1].index == 1)
+    opt = AdamW([torch.nn.Parameter(torch.zeros(4))])
+    with pytest.raises(RuntimeError, match="before the capture"):
+        opt._state_of(Parameter(), opt.param_groups[0])
