@@ -91,6 +91,11 @@ def _check_targets(logits, targets, mask, temperature):
         raise ValueError("more than 2^31 - 1 tokens, or 2^30 entries of the vocabulary")
 
 
+def _as_stored(*ts):
+    """Tensors that are what their memory holds: lazy negations are carried out."""
+    return tuple(None if t is None else t.resolve_neg() for t in ts)
+
+
 def _per_token(t, name, targets, strided=False):
     """A constant that goes with every token, in fp32; dense, or (strided) with strides for the sequence and the token."""
     _check_cuda(t)
@@ -102,7 +107,7 @@ def _per_token(t, name, targets, strided=False):
         raise ValueError(f"{name} {tuple(t.shape)} does not fit targets {tuple(targets.shape)}")
     if t.device != targets.device:
         raise ValueError(f"{name} must be on the logits' device")
-    t = t.detach().to(torch.float32)
+    t = _as_stored(t.detach())[0].to(torch.float32)
     return t if strided and t.dim() > 0 and (t.dim() <= 2 or t.is_contiguous()) else t.contiguous()
 
 
@@ -158,7 +163,7 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        return _logit_gradient(ctx, grad.to(torch.float32).contiguous(), 0), None, None, None
+        return _logit_gradient(ctx, _as_stored(grad)[0].to(torch.float32).contiguous(), 0), None, None, None
 
 
 def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, mask: torch.Tensor | None = None, *,
@@ -169,6 +174,7 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, mask: torch.Ten
     if lp is not None:
         return lp
     _check_targets(logits, targets, mask, temperature)
+    logits, targets, mask = _as_stored(logits, targets, mask)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _TokenLogProbs.apply(logits, targets, mask, temperature)
     return _log_probs(logits, targets, mask, temperature, False)[0]
@@ -221,7 +227,7 @@ class _PolicyLoss(torch.autograd.Function):
         g, ctx.g = ctx.g, None
         if g is not None and lib.wkv6_capture_id(_stream(g.device)) != ctx.capture:
             g = None
-        g = _logit_gradient(ctx, ctx.saved_tensors[4], 0, grad.to(torch.float32), g is not None, g)
+        g = _logit_gradient(ctx, ctx.saved_tensors[4], 0, _as_stored(grad)[0].to(torch.float32), g is not None, g)
         return g, None, None, None, None, None, None
 
 
@@ -253,6 +259,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
     if out is not None:
         return out
     _check_targets(logits, targets, mask, temperature)
+    logits, targets, mask = _as_stored(logits, targets, mask)
     consts = (_per_token(advantages, "advantages", targets, strided=True), _per_token(old_log_probs, "old_log_probs", targets),
               _per_token(ref_log_probs, "ref_log_probs", targets) if ref_log_probs is not None else None)
     args = (logits, targets, mask, temperature, consts, (clip_low, clip_high, kl_coef, scale), _REDUCTIONS[reduction])
@@ -293,7 +300,7 @@ class _PreferenceLoss(torch.autograd.Function):
     def backward(ctx, grad, _):
         if grad is None:
             return (None,) * 6
-        return _logit_gradient(ctx, ctx.saved_tensors[4], 1, grad.to(torch.float32)), None, None, None, None, None
+        return _logit_gradient(ctx, ctx.saved_tensors[4], 1, _as_stored(grad)[0].to(torch.float32)), None, None, None, None, None
 
 
 def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_log_probs: torch.Tensor | None = None,
@@ -317,6 +324,7 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_log_probs: 
     if out is not None:
         return out
     _check_targets(logits, targets, mask, 1.0)
+    logits, targets, mask = _as_stored(logits, targets, mask)
     ref = None if ref_log_probs is None else _per_token(ref_log_probs, "ref_log_probs", targets[:, 0] if targets.shape[1] else targets.sum(1))
     args = (logits, targets, mask, ref, (beta, label_smoothing, margin, scale), bool(average))
     if torch.is_grad_enabled() and logits.requires_grad:

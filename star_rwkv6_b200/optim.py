@@ -72,6 +72,8 @@ def _check_lists(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales):
                 raise ValueError("all tensors must be on one device")
             if l[i].layout != torch.strided or not l[i].is_contiguous():
                 raise ValueError(f"tensor {i} of a list is not contiguous")
+            if l[i].is_neg():
+                raise ValueError(f"tensor {i} of a list is lazily negated: what is written in place has to be what its memory holds")
     if _overlap([t for l in lists if l is not grads for t in l], grads):
         raise ValueError("parameters, moments and scales must not share memory, nor with gradients")
 
@@ -79,6 +81,8 @@ def _check_lists(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales):
 def _device_value(t, dtype, name, dev):
     if t.dtype != dtype or t.numel() != 1 or t.device != dev:
         raise ValueError(f"{name} must be one {dtype} value on the parameters' device")
+    if t.is_neg():
+        raise ValueError(f"{name} is lazily negated: it is read where it lies")
     return t.data_ptr()
 
 
@@ -104,6 +108,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp
     if _native.adamw_step(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales, step, lr, betas[0], betas[1], eps, weight_decay, seed,
                           bool(stochastic_rounding), grad_scale, first_index):
         return
+    grads = [g.resolve_neg() for g in grads]
     _check_lists(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales)
     if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
         raise ValueError("betas must lie in [0, 1)")
