@@ -23,7 +23,7 @@ import math
 import torch
 
 from ._lib import Policy, Preference, TokenLogits, check, lib
-from .ops import _DT, _check_cuda, _native, _ptr, _stream
+from .ops import _DT, _check_cuda, _check_tangents, _native, _ptr, _stream
 
 
 class _LMLoss(torch.autograd.Function):
@@ -92,7 +92,8 @@ def _check_targets(logits, targets, mask, temperature):
 
 
 def _as_stored(*ts):
-    """Tensors that are what their memory holds: lazy negations are carried out."""
+    """Tensors that are what their memory holds and no more: lazy negations are carried out, tangents refused."""
+    _check_tangents(*ts)
     return tuple(None if t is None else t.resolve_neg() for t in ts)
 
 
@@ -107,7 +108,7 @@ def _per_token(t, name, targets, strided=False):
         raise ValueError(f"{name} {tuple(t.shape)} does not fit targets {tuple(targets.shape)}")
     if t.device != targets.device:
         raise ValueError(f"{name} must be on the logits' device")
-    t = _as_stored(t.detach())[0].to(torch.float32)
+    t = _as_stored(t)[0].detach().to(torch.float32)
     return t if strided and t.dim() > 0 and (t.dim() <= 2 or t.is_contiguous()) else t.contiguous()
 
 

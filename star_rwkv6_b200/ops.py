@@ -106,6 +106,13 @@ def _check_cuda(*ts):
             raise RuntimeError("wkv6_b200 has no CPU path: all tensors must be CUDA tensors")
 
 
+def _check_tangents(*ts):
+    """For calls that do not go through an autograd node, which would refuse it."""
+    for t in ts:
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("forward-mode derivatives are not available here: the tangent of an argument would be lost")
+
+
 def resolve_variant(r, u, head_size: int, variant: int = _lib.VARIANT_AUTO) -> int:
     p = make_problem(r, u, head_size, out_dtype(r.dtype), variant)
     rc = lib.wkv6_resolve_variant(ctypes.byref(p))

@@ -13,7 +13,7 @@ import math
 import torch
 
 from ._lib import AdamWConfig, AdamWTensor, check, lib
-from .ops import _DT, _check_cuda, _native, _ptr, _stream
+from .ops import _DT, _check_cuda, _check_tangents, _native, _ptr, _stream
 
 BLOCK = 256      # values that share a scale where states have 8 bits
 BETA1 = 0.94     # the largest with 8 bits: above 17/18, first moments without gradients would never fall
@@ -52,6 +52,7 @@ def _check_lists(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales):
     dev = params[0].device
     for l in lists:
         _check_cuda(*l)
+        _check_tangents(*l)
     for i, p in enumerate(params):
         if p.dtype not in (torch.bfloat16, torch.float32):
             raise TypeError(f"parameter {i} must be bf16 or fp32, not {p.dtype}")
@@ -81,6 +82,7 @@ def _check_lists(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales):
 def _device_value(t, dtype, name, dev):
     if t.dtype != dtype or t.numel() != 1 or t.device != dev:
         raise ValueError(f"{name} must be one {dtype} value on the parameters' device")
+    _check_tangents(t)
     if t.is_neg():
         raise ValueError(f"{name} is lazily negated: it is read where it lies")
     return t.data_ptr()

@@ -1,5 +1,5 @@
 """Tensors that are not what their memory holds, or that carry more than a value: the losses and the optimizer step on lazily negated
-ones (the bits of the negated copy)."""
+ones (the bits of the negated copy), and on those with a forward-mode tangent (refused)."""
 import types
 
 import pytest
@@ -94,4 +94,53 @@ def test_lazily_negated_arguments_of_the_optimizer_step(path):
     codes = [torch.zeros(700, device="cuda").to(torch.float8_e4m3fn) for _ in range(2)]
     with pytest.raises(ValueError, match="negated"):
         adamw_step([p], [g], codes[:1], codes[1:], exp_avg_scales=[_lazily(s)], exp_avg_sq_scales=[s], step=2)
+    assert all(torch.equal(x, y) for x, y in zip((p, m, v), before))
+
+
+def _dual(x):
+    return torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x))
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_derivatives_of_the_losses_are_refused(path, grad_mode):
+    """Dual tensors do not require grad: their tangents must not be dropped on the path without a backward."""
+    given = list(_inputs())
+    want = _losses(*given)
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        for i in (0, 2, 3, 4, 5):
+            args = list(given)
+            args[i] = _dual(args[i])
+            for f in (lambda: _losses(*args)[0], lambda: _losses(*args)[1], lambda: _losses(*args)[3]):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    f()
+        assert all(torch.equal(a, b) for a, b in zip(_losses(*given), want))
+    for f in (lambda x: torch.func.jvp(lambda z: _losses(z, *given[1:])[0], (x,), (x,)), lambda x: torch.func.vmap(lambda z: _losses(z, *given[1:])[0])(x[None])):
+        with pytest.raises(RuntimeError):
+            f(given[0])
+
+
+def test_forward_mode_derivatives_of_the_gradients_are_refused(path):
+    z, *rest = _inputs()
+    z.requires_grad_(True)
+    outs = _losses(z, *rest)
+    with torch.autograd.forward_ad.dual_level():
+        for i in (0, 1, 3):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(outs[i], z, _dual(torch.ones_like(outs[i])))
+
+
+def test_forward_mode_derivatives_of_the_optimizer_step_are_refused(path):
+    from star_rwkv6_b200.optim import adamw_step
+    p, g, m, v = _state()
+    before = [x.clone() for x in (p, m, v)]
+    one = torch.ones((), device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        for i in range(4):
+            lists = [[p], [g], [m], [v]]
+            lists[i] = [_dual(lists[i][0])]
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                adamw_step(*lists, step=1)
+        for kw in (dict(lr=_dual(one)), dict(grad_scale=_dual(one))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                adamw_step([p], [g], [m], [v], step=1, **kw)
     assert all(torch.equal(x, y) for x, y in zip((p, m, v), before))
