@@ -448,7 +448,7 @@ struct Policy {
     int reduction;
     const int *counts;       // live rows of each part
     int parts;
-    float *row_loss;         // of each block
+    double *row_loss;        // of each block
     unsigned *done;
     float *loss;
 };
@@ -469,7 +469,7 @@ __device__ __forceinline__ void total_loss(const Policy &q, const bool &last) {
     if (!last) return;
     __threadfence();
     double x = 0.0;
-    for (unsigned i = threadIdx.x; i < gridDim.x; i += blockDim.x) x += (double)__ldcg(q.row_loss + i);
+    for (unsigned i = threadIdx.x; i < gridDim.x; i += blockDim.x) x += __ldcg(q.row_loss + i);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = x;
@@ -567,7 +567,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 32 * kWarpRows : THREADS, Long
 token_rows_kernel(const Rows a, float *__restrict__ lp_out, float2 *__restrict__ stat, const Policy q, float *__restrict__ coefficient,
                   T *__restrict__ g) {
     __shared__ bool last;
-    __shared__ float of_warp[kWarpRows];
+    __shared__ double of_warp[kWarpRows];
     const int tid = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x;
     const int64_t row = THREADS == 32 ? (int64_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5) : blockIdx.x;
     if (THREADS != 32 || row < a.rows) {
@@ -627,7 +627,7 @@ token_rows_kernel(const Rows a, float *__restrict__ lp_out, float2 *__restrict__
         if constexpr (THREADS == 32) {
             __syncthreads();
             if (threadIdx.x == 0) {
-                float x = 0.f;
+                double x = 0.0;
                 for (int i = 0; i < kWarpRows; ++i)
                     if (blockIdx.x * (int64_t)kWarpRows + i < a.rows) x += of_warp[i];
                 q.row_loss[blockIdx.x] = x;
@@ -917,7 +917,7 @@ extern "C" uint64_t wkv6_capture_id(void *stream) {
 
 extern "C" size_t wkv6_policy_loss_workspace_bytes(int32_t S, int32_t T, int32_t reduction) {
     if (S <= 0 || T <= 0) return 0;
-    return 16 + (size_t)((int64_t)S * T) * 4 + (size_t)count_parts(S, T, reduction) * 4;
+    return 16 + (size_t)((int64_t)S * T) * 8 + (size_t)count_parts(S, T, reduction) * 4;
 }
 
 extern "C" int wkv6_policy_loss(const wkv6_token_logits *p, const wkv6_policy *c, float *loss, float *log_probs, float *stat,
@@ -953,7 +953,7 @@ extern "C" int wkv6_policy_loss(const wkv6_token_logits *p, const wkv6_policy *c
     q.scale = (float)c->scale;
     q.reduction = c->reduction;
     q.done = static_cast<unsigned *>(workspace);
-    q.row_loss = reinterpret_cast<float *>(static_cast<char *>(workspace) + 16);
+    q.row_loss = reinterpret_cast<double *>(static_cast<char *>(workspace) + 16);
     int *counts = reinterpret_cast<int *>(q.row_loss + a.rows);
     q.counts = counts;
     q.parts = (int)count_parts(p->S, p->T, c->reduction);
