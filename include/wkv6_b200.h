@@ -241,7 +241,8 @@ WKV6_API int wkv6_scale_bf16(int64_t n, void *g, const float *scale, void *strea
  * logits + s * seq_stride + t * row_stride (elements; 0 selects the dense value), the rest is dense [S, T].
  *   lp = z_a / temperature - log sum_j exp(z_j / temperature), fp32 arithmetic
  * A token whose mask is 0 or whose target lies outside [0, V) does not count: its logits are not read, its log-probability is 0, and
- * its gradient is zeros.  Gradients are dense [S, T, V] of `dtype` and must not overlap the logits.
+ * its gradient is zeros.  Gradients are dense [S, T, V] of `dtype`, 16-byte aligned, and must not overlap the logits; every other array is
+ * aligned to its elements.
  */
 typedef struct {
     int32_t S, T, V;                     /* S * T < 2^31, V <= 2^30 */

@@ -517,6 +517,8 @@ extern "C" int wkv6_adamw_step(const wkv6_adamw *c, int64_t count, const wkv6_ad
     if (!(c->beta1 >= 0.0 && c->beta1 < 1.0 && c->beta2 >= 0.0 && c->beta2 < 1.0)) return fail(WKV6_ERR_INVALID, "wkv6_adamw_step: betas must lie in [0, 1)");
     // without gradients a code falls only if beta1 of it is beyond the border to its lower neighbour, which is at 17/18 of a code 1.125 2^n
     if (c->state_bits == 8 && c->beta1 > 0.94) return fail(WKV6_ERR_UNSUPPORTED, "wkv6_adamw_step: beta1 = %g, at most 0.94 with states of 8 bits", c->beta1);
+    if (!aligned(8, {c->step_device}) || !aligned(4, {c->lr_device, c->grad_scale}))
+        return fail(WKV6_ERR_INVALID, "wkv6_adamw_step: values on the device must be aligned to their size");
     const size_t e = dtype_size(c->dtype), es = c->state_bits == 32 ? 4 : 1;
     for (int64_t i = 0; i < count; ++i) {
         const wkv6_adamw_tensor &t = ts[i];

@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "../../include/wkv6_b200.h"
 
 namespace wkv6 {
@@ -17,6 +19,11 @@ struct Dims {
 };
 
 int sm_count();   // of the current device
+inline bool aligned(size_t bytes, std::initializer_list<const void *> ps) {
+    for (const void *p : ps)
+        if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
+    return true;
+}
 inline bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 int fail(int code, const char *fmt, ...);
 int cuda_fail(cudaError_t e, const char *what);

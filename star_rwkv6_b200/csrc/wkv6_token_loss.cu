@@ -837,6 +837,7 @@ int rows_of(const wkv6_token_logits *p, Rows *a, const char *what, bool need_log
     if (a->row_stride < 0 || a->seq_stride < 0) return fail(WKV6_ERR_INVALID, "%s: negative strides", what);
     if (a->rows > 0 && ((need_logits && p->logits == nullptr) || p->targets == nullptr)) return fail(WKV6_ERR_INVALID, "%s: NULL argument", what);
     if (reinterpret_cast<uintptr_t>(p->logits) % dtype_size(p->dtype)) return fail(WKV6_ERR_INVALID, "%s: misaligned logits", what);
+    if (!aligned(8, {p->targets})) return fail(WKV6_ERR_INVALID, "%s: misaligned targets", what);
     a->z = p->logits;
     a->targets = p->targets;
     a->mask = p->mask;
@@ -879,7 +880,7 @@ extern "C" int wkv6_token_log_probs(const wkv6_token_logits *p, float *log_probs
     if (const int rc = rows_of(p, &a, "wkv6_token_log_probs", true)) return rc;
     if (a.rows == 0) return WKV6_OK;
     if (log_probs == nullptr) return fail(WKV6_ERR_INVALID, "wkv6_token_log_probs: NULL argument");
-    if (reinterpret_cast<uintptr_t>(stat) % 8) return fail(WKV6_ERR_INVALID, "wkv6_token_log_probs: stat must be 8-byte aligned");
+    if (!aligned(8, {stat}) || !aligned(4, {log_probs})) return fail(WKV6_ERR_INVALID, "wkv6_token_log_probs: stat must be 8-byte aligned, log_probs 4-byte");
     return launch_rows<false>(p, a, log_probs, reinterpret_cast<float2 *>(stat), Policy{}, nullptr, nullptr, static_cast<cudaStream_t>(stream));
 }
 
@@ -889,8 +890,8 @@ extern "C" int wkv6_token_log_probs_backward(const wkv6_token_logits *p, const f
     if (const int rc = rows_of(p, &a, "wkv6_token_log_probs_backward", true)) return rc;
     if (a.rows == 0) return WKV6_OK;
     if (!stat || !coefficient || !g || (unless_one && !factor)) return fail(WKV6_ERR_INVALID, "wkv6_token_log_probs_backward: NULL argument");
-    if (!aligned16(g) || reinterpret_cast<uintptr_t>(stat) % 8)
-        return fail(WKV6_ERR_INVALID, "wkv6_token_log_probs_backward: the gradient must be 16-byte aligned, stat 8-byte");
+    if (!aligned16(g) || !aligned(8, {stat}) || !aligned(4, {coefficient, factor}))
+        return fail(WKV6_ERR_INVALID, "wkv6_token_log_probs_backward: the gradient must be 16-byte aligned, stat 8-byte, other values 4-byte");
     return dispatch(p, true, [&](auto size, auto *t) {
         using T = std::remove_pointer_t<decltype(t)>;
         constexpr int threads = size.value;
@@ -934,8 +935,9 @@ extern "C" int wkv6_policy_loss(const wkv6_token_logits *p, const wkv6_policy *c
     }
     if (!c->advantages || !c->old_log_probs || !log_probs || !coefficient || !workspace)
         return fail(WKV6_ERR_INVALID, "wkv6_policy_loss: NULL argument");
-    if (!aligned16(g) || reinterpret_cast<uintptr_t>(stat) % 8 || !aligned16(workspace))
-        return fail(WKV6_ERR_INVALID, "wkv6_policy_loss: the gradient and the workspace must be 16-byte aligned, stat 8-byte");
+    if (!aligned16(g) || !aligned(8, {stat}) || !aligned16(workspace) ||
+        !aligned(4, {loss, log_probs, coefficient, c->advantages, c->old_log_probs, c->ref_log_probs}))
+        return fail(WKV6_ERR_INVALID, "wkv6_policy_loss: the gradient and the workspace must be 16-byte aligned, stat 8-byte, other values 4-byte");
     if (workspace_bytes < wkv6_policy_loss_workspace_bytes(p->S, p->T, c->reduction))
         return fail(WKV6_ERR_WORKSPACE, "wkv6_policy_loss: workspace of %zu bytes, %zu are needed", workspace_bytes,
                     wkv6_policy_loss_workspace_bytes(p->S, p->T, c->reduction));
@@ -979,7 +981,8 @@ extern "C" int wkv6_preference_loss(const wkv6_token_logits *p, const float *log
     }
     if (!sequence_log_probs || !coefficient || !workspace || (a.rows && !log_probs))
         return fail(WKV6_ERR_INVALID, "wkv6_preference_loss: NULL argument");
-    if (reinterpret_cast<uintptr_t>(workspace) % 8) return fail(WKV6_ERR_INVALID, "wkv6_preference_loss: the workspace must be 8-byte aligned");
+    if (!aligned(8, {workspace}) || !aligned(4, {log_probs, c->ref_log_probs, loss, sequence_log_probs, coefficient}))
+        return fail(WKV6_ERR_INVALID, "wkv6_preference_loss: the workspace must be 8-byte aligned, other values 4-byte");
     if (workspace_bytes < wkv6_preference_loss_workspace_bytes(p->S))
         return fail(WKV6_ERR_WORKSPACE, "wkv6_preference_loss: workspace of %zu bytes, %zu are needed", workspace_bytes,
                     wkv6_preference_loss_workspace_bytes(p->S));
