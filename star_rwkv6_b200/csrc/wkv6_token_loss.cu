@@ -1000,8 +1000,10 @@ extern "C" int wkv6_preference_loss(const wkv6_token_logits *p, const float *log
     q.count = reinterpret_cast<int *>(q.seq64 + p->S);
     q.coefficient = coefficient;
     q.loss = loss;
-    // one block against two launches: 3.1 and 3.8 us at 2 x 65, 5.0 and 4.6 at 8 x 1024, 7.1 and 4.5 at 32 x 700, 9.3 and 4.5 at 128 x 64
-    if (p->S <= 32 && p->T <= 1024) {
+    // One block against two launches, us per call of the whole loss without gradient (V = 40) and, behind it, of its replay in a graph:
+    // 2 x 65 tokens 8.7 and 12.3 (5.2 and 6.2), 8 x 512 10.3 and 12.3 (7.2 and 7.2), 32 x 128 10.3 and 12.3 (7.3 and 7.1); but 2 x 1024
+    // 10.3 and 12.3 (8.3 and 6.9), 8 x 1024 14.4 and 14.4 (10.3 and 8.3), 32 x 300 14.4 and 14.4 (10.8 and 9.0), 32 x 1024 23.6 and 21.5.
+    if (p->S <= 32 && p->T <= 512 && (int64_t)p->S * p->T <= 4096) {
         preference_kernel<<<1, kOneBlock, 0, st>>>(a, q);
     } else {
         sequence_sum_kernel<<<p->S, 256, 0, st>>>(a, q);
