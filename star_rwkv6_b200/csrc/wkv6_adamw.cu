@@ -454,7 +454,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) adamw_kernel(const __g
     }
 }
 
-// Tensors of one launch: what fits into the 32764 bytes of arguments, or a small table where that is enough (its launch is cheaper).
+// Tensors of one launch: what fits into the 32764 bytes of arguments, or a small table where that is enough: its launch is cheaper (calls
+// of 16 tensors of 1000 values 6 us, 8 with the large table; of 54 tensors 12.2 and 14.2; a replayed launch takes 5.1 and 5.6 us either way).
 constexpr int kTensors = 500, kFewTensors = 56;
 
 template <typename T, int BITS, bool STOCHASTIC, int CAP>
