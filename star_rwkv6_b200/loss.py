@@ -45,7 +45,7 @@ class _LMLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
         (g,) = ctx.saved_tensors
-        scale = grad_out.to(torch.float32)
+        scale = grad_out.resolve_neg().to(torch.float32)
         with torch.cuda.device(g.device):      # in place: the buffer is this function's own; nothing moves for a factor of 1
             check(lib.wkv6_scale_bf16(g.numel(), _ptr(g), _ptr(scale), _stream(g.device)))
         torch.autograd.graph.increment_version(g)      # a second backward would scale it again: autograd refuses that
@@ -55,7 +55,7 @@ class _LMLoss(torch.autograd.Function):
 def lm_loss(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     """Mean cross-entropy of bf16 ``logits`` [..., V] against int64 ``targets`` [...]; overwrites ``logits``."""
     V = logits.shape[-1]
-    if logits.dtype != torch.bfloat16 or V % 8 or V > 65536 or not logits.is_contiguous():
+    if logits.dtype != torch.bfloat16 or V % 8 or V > 65536 or not logits.is_contiguous() or logits.is_neg():
         # same definition as the fused kernel: rows whose target lies outside [0, V) give zero loss and gradient,
         # and the mean runs over all rows
         z, t = logits.float().reshape(-1, V), targets.reshape(-1)
@@ -63,7 +63,7 @@ def lm_loss(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         per_row = torch.nn.functional.cross_entropy(z, t.clamp(0, V - 1), reduction="none") * valid
         return per_row.sum() / max(z.shape[0], 1)
     _check_cuda(logits, targets)
-    return _LMLoss.apply(logits, targets)
+    return _LMLoss.apply(logits, targets.resolve_neg())
 
 
 def _check_targets(logits, targets, mask, temperature):

@@ -144,3 +144,14 @@ def test_forward_mode_derivatives_of_the_optimizer_step_are_refused(path):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 adamw_step([p], [g], [m], [v], step=1, **kw)
     assert all(torch.equal(x, y) for x, y in zip((p, m, v), before))
+
+
+def test_the_next_token_loss_of_lazily_negated_tensors():
+    from star_rwkv6_b200.loss import lm_loss
+    z = torch.randn(4, 64, device="cuda").bfloat16()
+    t = torch.arange(4, device="cuda")
+    x, y = torch.neg(z).requires_grad_(True), z.clone().requires_grad_(True)
+    a, b = lm_loss(torch._neg_view(x), t), lm_loss(y * 1, t)
+    assert abs(a.item() - b.item()) <= 2 * 2.5e-6 + 2.0 ** -22 * b.item()        # two forms, each as in test_token_losses.py
+    (ga,), (gb,) = torch.autograd.grad(a, x), torch.autograd.grad(b, y, _lazily(torch.full((), 1.0, device="cuda")))
+    assert (ga.float() + gb.float()).abs().max() <= 2.0 ** -8 * gb.abs().max() and gb.any() and torch.equal(x, -z)
