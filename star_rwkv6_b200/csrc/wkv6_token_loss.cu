@@ -1000,10 +1000,11 @@ extern "C" int wkv6_preference_loss(const wkv6_token_logits *p, const float *log
     q.count = reinterpret_cast<int *>(q.seq64 + p->S);
     q.coefficient = coefficient;
     q.loss = loss;
-    // One block against two launches, us per call of the whole loss without gradient (V = 40) and, behind it, of its replay in a graph:
-    // 2 x 65 tokens 8.7 and 12.3 (5.2 and 6.2), 8 x 512 10.3 and 12.3 (7.2 and 7.2), 32 x 128 10.3 and 12.3 (7.3 and 7.1); but 2 x 1024
-    // 10.3 and 12.3 (8.3 and 6.9), 8 x 1024 14.4 and 14.4 (10.3 and 8.3), 32 x 300 14.4 and 14.4 (10.8 and 9.0), 32 x 1024 23.6 and 21.5.
-    if (p->S <= 32 && p->T <= 512 && (int64_t)p->S * p->T <= 4096) {
+    // One block against two launches.  A training call of few rows' bytes is bound by the host, which the second launch costs 2 us: forward and
+    // gradient of 32 x 700 tokens, V = 259, 62.7 us and 64.6, 32 x 1024 62.7 and 64.3, 2 x 65 62.7 and 64.0.  What the rule gives up is device
+    // time where the host waits or a graph is replayed: 32 x 700 33.1 us and 29.9, 8 x 1024 18.0 and 16.1, 32 x 1024 45.4 and 40.7, while up to
+    // 4096 tokens there is nothing to give up (8 x 512 12.9 and 12.9, 32 x 128 12.9 and 12.7, 2 x 65 of 65536 bf16 16.6 and 17.4).
+    if (p->S <= 32 && p->T <= 1024) {
         preference_kernel<<<1, kOneBlock, 0, st>>>(a, q);
     } else {
         sequence_sum_kernel<<<p->S, 256, 0, st>>>(a, q);

@@ -8,7 +8,7 @@ from test_token_losses import LP, _np
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("S,T", [(8, 512), (8, 513), (32, 128), (32, 129), (34, 120), (2, 512), (2, 513), (32, 1), (34, 1), (2, 1025)])
+@pytest.mark.parametrize("S,T", [(8, 512), (8, 513), (32, 128), (32, 129), (34, 120), (2, 512), (2, 513), (32, 1), (34, 1), (2, 1025), (32, 1024), (34, 1024)])
 @pytest.mark.parametrize("average", [False, True])
 def test_on_both_sides(S, T, average):
     from star_rwkv6_b200.loss import preference_loss
