@@ -53,6 +53,9 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// (a - b) k, by way of half the difference: that of two values at the ends of the range does not overflow, and k may be small.
+__device__ __forceinline__ float apart(float a, float b, float k) { return fmaf(a, 0.5f, -0.5f * b) * (2.f * k); }
+
 // Sixteen bytes of logits as fp32 pairs and back (each value rounded once, to nearest).
 template <typename T> struct Vec;
 
@@ -180,7 +183,7 @@ __device__ __forceinline__ void take(const uint4 (&q)[U], float k, Part &r, int 
 // kernels that come here give the same bits.)  WIDE: c is the maximum itself.
 template <typename T, bool WIDE>
 __device__ __forceinline__ float gradient_of(float z, float k, float c, float neg) {
-    return __fmul_rn(ex2(WIDE ? (z - c) * k : fmaf(z, k, -c)), neg);
+    return __fmul_rn(ex2(WIDE ? apart(z, c, k) : fmaf(z, k, -c)), neg);
 }
 template <typename T, bool WIDE>
 __device__ __forceinline__ uint4 gradient_of(const uint4 &q, int at, float k, float c, float neg, float g) {
@@ -399,7 +402,7 @@ __device__ __forceinline__ void row_part_wide(const T *z, int V, int first, int 
     sum = 0.f;
     for (int i = first; i < V; i += step) {
         const float x = Vec<T>::get1(z[i]), m = fmaxf(mx, x);
-        sum = sum * ex2((mx - m) * k) + ex2((x - m) * k);
+        sum = sum * ex2(apart(mx, m, k)) + ex2(apart(x, m, k));
         mx = m;
     }
 }
@@ -408,7 +411,7 @@ __device__ __forceinline__ void row_part_wide(const T *z, int V, int first, int 
 template <int THREADS, int TURN>
 __device__ __forceinline__ void gather(float &c, float &sum, float k) {
     const float m = warp_max(c);
-    sum = warp_sum(sum * ex2((c - m) * k));
+    sum = warp_sum(sum * ex2(apart(c, m, k)));
     c = m;
     if constexpr (THREADS != 32) {
         __shared__ float2 part[THREADS / 32];
@@ -417,7 +420,7 @@ __device__ __forceinline__ void gather(float &c, float &sum, float k) {
         __syncthreads();
         const float2 p = lane < THREADS / 32 ? part[lane] : make_float2(c, 0.f);
         c = warp_max(p.x);
-        sum = warp_sum(p.y * ex2((p.x - c) * k));
+        sum = warp_sum(p.y * ex2(apart(p.x, c, k)));
     }
 }
 
@@ -548,8 +551,7 @@ __device__ __forceinline__ float finish_row(const Rows &a, const T *z, float zt,
     if (wide) {
         row_part_wide(z, a.V, tid, THREADS, a.k, r.c, r.sum);
         gather<THREADS, 1>(r.c, r.sum, a.k);
-        const float below = zt - r.c;      // overflows between the ends of the type's range
-        return at_most_zero((below == -INFINITY ? zt * a.inv_tau - r.c * a.inv_tau : below * a.inv_tau) - logf(r.sum));
+        return at_most_zero(apart(zt, r.c, a.inv_tau) - logf(r.sum));
     }
     const float below = fmaf(zt, a.k, -r.c);
     if (below == -INFINITY) return zt * a.inv_tau + (r.sum - r.sum);      // the type's lowest value: its product with log2(e) leaves fp32, the rest is lost in it

@@ -36,7 +36,8 @@ def _check(z, targets, tau=1.0, both_losses=True):
     S, T, V = z.shape
     g = torch.Generator().manual_seed(V)
     up, adv, noise = (torch.randn(S, T, generator=g) for _ in range(3))
-    up = up * tau
+    scale = min(tau, 1e37)       # gradients and losses times 3e38 would be infinite, an input of which nothing follows
+    up = up * scale
     zc = z.cuda().requires_grad_(True)
     t = targets.cuda()
     lp, p, live = O.log_probs(_np(z), _np(targets), None, tau)
@@ -48,14 +49,14 @@ def _check(z, targets, tau=1.0, both_losses=True):
     near = lp > -50
     old = torch.from_numpy(np.where(near, lp + 0.3 * _np(noise), 0.0)).float()
     for backward in (True, False):
-        loss, want_lp, want, c = O.policy(_np(z), _np(targets), _np(adv), _np(old), tau=tau, scale=tau)
+        loss, want_lp, want, c = O.policy(_np(z), _np(targets), _np(adv), _np(old), tau=tau, scale=scale)
         with torch.set_grad_enabled(backward):
-            got, got_lp = policy_loss(zc, t, adv.cuda(), old.cuda(), temperature=tau, scale=tau)
+            got, got_lp = policy_loss(zc, t, adv.cuda(), old.cuda(), temperature=tau, scale=scale)
         _close(got_lp, want_lp, ABS + REL * np.abs(want_lp))
-        sizes = O.policy(_np(z), _np(targets), np.abs(_np(adv)), _np(old), None, None, 0.999, 1e9, tau=tau, scale=tau)[0]
+        sizes = O.policy(_np(z), _np(targets), np.abs(_np(adv)), _np(old), None, None, 0.999, 1e9, tau=tau, scale=scale)[0]
         # the clipped value of a ratio near zero is not among those sizes
-        _close(got, loss, RATIO * (abs(sizes) + tau * float(adv.abs().mean())) + 2.0 ** -22 * abs(loss))
-    loss, _ = policy_loss(zc, t, adv.cuda(), old.cuda(), temperature=tau, scale=tau)
+        _close(got, loss, RATIO * (abs(sizes) + scale * float(adv.abs().mean())) + 2.0 ** -22 * abs(loss))
+    loss, _ = policy_loss(zc, t, adv.cuda(), old.cuda(), temperature=tau, scale=scale)
     (gz,) = torch.autograd.grad(loss, zc, retain_graph=True)
     _gradient_close(gz, want, c / tau, z.dtype, RATIO)
     (again,) = torch.autograd.grad(loss * 2, zc)            # from the kept statistics
@@ -164,3 +165,38 @@ def test_a_chosen_token_at_the_types_lowest_value(V, dtype):
     (gz,) = torch.autograd.grad(loss, zc)
     assert loss.isfinite() and gz.isfinite().all()
     _gradient_close(gz, want, c[:, None], dt, 2.0 ** -22)        # |D| is above 1000: the slope is saturated
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_an_impossible_token_in_a_row_at_the_types_lowest_value(dtype):
+    """-inf, whatever the temperature makes of the row's maximum; in a row of nothing but -inf NaN."""
+    from star_rwkv6_b200.loss import policy_loss, token_log_probs
+    z = torch.full((4, 333), torch.finfo(TYPES[dtype]).min, dtype=TYPES[dtype], device="cuda")
+    z[:, 7] = float("-inf")
+    z[1, 1], z[2, 9] = 3.0, torch.finfo(TYPES[dtype]).max
+    z[3] = float("-inf")
+    z.requires_grad_(True)
+    t = torch.full((4,), 7, device="cuda")
+    for tau in (1.0, 0.7, 1e-20, 1e-30, 7.0, 1e38):
+        lp = token_log_probs(z, t, temperature=tau)
+        assert lp[:3].isneginf().all() and lp[3].isnan()
+        loss, again = policy_loss(z, t, torch.ones(4, device="cuda"), torch.zeros(4, device="cuda"), mask=lp.isneginf(), temperature=tau)
+        assert again[:3].isneginf().all() and loss == 0 and not torch.autograd.grad(loss, z)[0].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [40, 4099, 20001])
+def test_both_ends_of_the_range_at_large_temperatures(V, dtype):
+    """Values at both ends of the type's range are a few units apart at a temperature of 3e38: their difference is more than fp32 holds."""
+    most = torch.finfo(TYPES[dtype]).max
+    g = torch.Generator().manual_seed(V + 3)
+    z = torch.where(torch.rand(2, 5, V, generator=g) < 0.5, most, -most)
+    z[:, 1] = 3 * torch.randn(2, V, generator=g)
+    z[:, 1, 3::7] = -most
+    z[:, 2, 1:] = -most
+    z[:, 2, 0] = most
+    at = torch.randint(0, V, (2, 5), generator=g)
+    for tau in (3e38, 1e38, 2e37):
+        _check(z.to(TYPES[dtype]), at, tau)
