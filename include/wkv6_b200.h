@@ -309,7 +309,7 @@ WKV6_API int wkv6_preference_loss(const wkv6_token_logits *p, const float *log_p
  * be at most 0.94 with 8 bits).  stochastic: bf16 parameters are rounded the same way, from 16 random bits each; otherwise to nearest.  The random bits are
  * a function of the lowest 32 bits of seed and t, the tensor's `index` and the value's place in it.
  * A gradient that is infinite or NaN makes its value NaN (8 bits: its block's moments too).
- * t is `step`, or *step_device where that is not NULL (at least 1); lr is `lr`, or *lr_device.  Tensors must not overlap; n == 0 is allowed.
+ * eps is 0 or a normal fp32 number.  t is `step`, or *step_device where that is not NULL (at least 1); lr is `lr`, or *lr_device.  Tensors must not overlap; n == 0 is allowed.
  * No counterpart in the reference (its trainer files are empty).
  */
 typedef struct {

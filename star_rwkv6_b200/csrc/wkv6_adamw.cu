@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 
@@ -516,6 +517,8 @@ extern "C" int wkv6_adamw_step(const wkv6_adamw *c, int64_t count, const wkv6_ad
     if (c->state_bits != 8 && c->state_bits != 32) return fail(WKV6_ERR_UNSUPPORTED, "wkv6_adamw_step: states of %d bits", c->state_bits);
     if (c->step_device == nullptr && c->step < 1) return fail(WKV6_ERR_INVALID, "wkv6_adamw_step: step must be at least 1");
     if (!(c->beta1 >= 0.0 && c->beta1 < 1.0 && c->beta2 >= 0.0 && c->beta2 < 1.0)) return fail(WKV6_ERR_INVALID, "wkv6_adamw_step: betas must lie in [0, 1)");
+    if (!(c->eps == 0.0 || (c->eps >= (double)FLT_MIN && c->eps <= (double)FLT_MAX)))      // a subnormal one would be zero in reciprocal()
+        return fail(WKV6_ERR_INVALID, "wkv6_adamw_step: eps must be 0 or a normal fp32 number, not %g", c->eps);
     // without gradients a code falls only if beta1 of it is beyond the border to its lower neighbour, which is at 17/18 of a code 1.125 2^n
     if (c->state_bits == 8 && c->beta1 > 0.94) return fail(WKV6_ERR_UNSUPPORTED, "wkv6_adamw_step: beta1 = %g, at most 0.94 with states of 8 bits", c->beta1);
     if (!aligned(8, {c->step_device}) || !aligned(4, {c->lr_device, c->grad_scale}))

@@ -8,6 +8,7 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <vector>
 
@@ -500,7 +501,7 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
     const at::ScalarType state = narrow ? at::kFloat8_e4m3fn : at::kFloat;
     wkv6_adamw c{};
     double x[4];
-    if (!numbers(args + 8, 4, x) || !(x[0] >= 0.0 && x[0] < 1.0 && x[1] >= 0.0 && x[1] < 1.0) || !(x[2] >= 0.0) || std::isinf(x[2]) || !std::isfinite(x[3]))
+    if (!numbers(args + 8, 4, x) || !(x[0] >= 0.0 && x[0] < 1.0 && x[1] >= 0.0 && x[1] < 1.0) || !(x[2] == 0.0 || (x[2] >= FLT_MIN && x[2] <= FLT_MAX)) || !std::isfinite(x[3]))
         return none();
     c.state_bits = narrow ? 8 : 32;
     if (narrow && x[0] > 0.94) return none();

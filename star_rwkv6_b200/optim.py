@@ -19,6 +19,12 @@ BLOCK = 256      # values that share a scale where states have 8 bits
 BETA1 = 0.94     # the largest with 8 bits: above 17/18, first moments without gradients would never fall
 
 
+def _check_eps(eps):
+    fp32 = torch.finfo(torch.float32)
+    if not (eps == 0.0 or fp32.tiny <= eps <= fp32.max):
+        raise ValueError(f"eps must be 0 or a normal fp32 number, not {eps}")
+
+
 def _check_beta1(state_bits, beta1):
     if state_bits == 8 and beta1 > BETA1:
         raise ValueError(f"states in 8 bits take beta1 up to {BETA1}, not {beta1}: first moments are rounded to nearest and would not move")
@@ -115,8 +121,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, exp_avg_scales=None, exp
     if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
         raise ValueError("betas must lie in [0, 1)")
     _check_beta1(32 if m_scales is None else 8, betas[0])
-    if not (math.isfinite(eps) and eps >= 0.0 and math.isfinite(weight_decay)):
-        raise ValueError("eps must not be negative, eps and weight_decay must be finite")
+    _check_eps(eps)
+    if not math.isfinite(weight_decay):
+        raise ValueError("weight_decay must be finite")
     if not params:
         return
     if not 0 <= first_index <= 2 ** 31 - len(params):
@@ -186,8 +193,9 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("lr must be finite and not negative")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
             raise ValueError("betas must lie in [0, 1)")
-        if not (math.isfinite(eps) and eps >= 0.0 and math.isfinite(weight_decay) and weight_decay >= 0.0):
-            raise ValueError("eps and weight_decay must be finite and not negative")
+        _check_eps(eps)
+        if not (math.isfinite(weight_decay) and weight_decay >= 0.0):
+            raise ValueError("weight_decay must be finite and not negative")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       stochastic_rounding=stochastic_rounding, seed=seed, capturable=capturable, step=None))
 
