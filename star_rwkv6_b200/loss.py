@@ -13,6 +13,7 @@ The gradient is written over the logits inside the forward call: the logits tens
 sampled or compared answers.  They leave the logits alone, take bf16, fp16 and fp32 logits of any vocabulary, and compute in fp32.
 Tokens that ``mask`` leaves out, and those whose target lies outside [0, V), do not count: their logits are not read, their
 log-probability is 0 and their gradient zeros.  A row that counts and holds a NaN or +inf, or nothing but -inf, gives NaN.
+Temperatures of at least 1e-30 and finite logits of any size are computed as written; forward-mode derivatives are refused.
 Forward and backward can be captured into a CUDA graph; as with every backward pass, no eager graph of the same leaves may be alive then.
 """
 from __future__ import annotations

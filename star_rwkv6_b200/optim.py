@@ -181,6 +181,7 @@ class AdamW(torch.optim.Optimizer):
     ``grad_scale``: an attribute, None or one fp32 value on the device that multiplies the gradients of the next steps.
     ``capturable``: the step number is kept on the device (one per group), so that ``step`` can be captured into a CUDA graph; every
     parameter that gets gradients must then get them from its group's first step on.  A float ``lr`` stays in a captured step as it was.
+    A group whose ``capturable`` is set or cleared later goes on from its step; that next step has to lie outside of a capture.
     ``state_dict`` holds the moments in their own types; ``load_state_dict`` keeps them (parameters do not lend them theirs)."""
 
     grad_scale = None       # of the class: copies and unpickled optimizers do not go through __init__
